@@ -523,6 +523,83 @@ int mosaic_dsa_kv_write(const uint16_t* kv, const int32_t* slots, int64_t rows, 
 int mosaic_dsa_decode_indices(const int32_t* pos, int64_t rows, int64_t window, const int32_t* cidx, int64_t nc,
                               int64_t ratio, int64_t offset, int32_t* out, void* stream);
 
+/* ----------------------------------------------------- paged KV cache ---- */
+/* One pool of pages holds the keys and values of many requests in 8 bits:
+ * codes [pages, blocks, kv_heads, 2, 64 head_dim] e4m3 and scales [pages,
+ * blocks, kv_heads, 2] e8m0 (the value is code * 2^(scale - 127)).  A page is
+ * `blocks` (1..64) blocks of 64 tokens, page_size = 64 blocks; index 0 of the
+ * last but one axis holds keys, 1 values.  The bytes of a block are
+ *   keys   [4 tg][head_dim/64 dg][4 q][16 c][16 j]: token 16 tg + c, dim 64 dg + 16 q + j
+ *   values [head_dim/16 dt][4 q][16 c][4 w][4 j]:   token 16 w + 4 q + j, dim 16 dt + c
+ * A batch is `requests` runs of token rows: request r's rows of this call are
+ * starts[r] .. starts[r + 1] (ascending, starts[0] = 0), its tokens with them
+ * number seq_lens[r], and its pages are row r of block_table (row stride
+ * table_stride, width entries).  All index arrays are int32.  Page ids outside
+ * the pool, and starts outside the token rows, are never followed.  The
+ * reference keeps one contiguous cache for each sequence
+ * (mosaicvm/model/dsa_layers.py:393-400); it has no counterpart of these. */
+
+/* Block tables and slot map of one step.  lengths [requests]: tokens that each
+ * request holds; add [requests]: tokens that this step adds (negative: none).
+ * Requests are placed in order; one is not placed where its rows pass `tokens`,
+ * its tokens pass its table row, or the pool has too few pages left.  A placed
+ * request's new pages are popped from the stack free_pages[0 .. *free_count)
+ * (top: the last one) into its table row; with free_pages NULL the tables hold
+ * them already.  Outputs: starts [requests + 1] (the prefix of add, placed or
+ * not, cut at tokens); lengths_out [requests]; seq_lens [requests] = lengths_out
+ * where placed and 0 where not (the reader and writer below then skip the
+ * request: its rows attend to nothing and give zeros); positions and slots
+ * [tokens] (page id * page_size + offset; -1 for rows that are not placed or
+ * behind the last request); *count_out: pages left.  Outputs may not overlap
+ * inputs (block_table is updated in place).  tokens < 2^21, requests <= 2^20,
+ * page_size a multiple of 64 up to 4096, pages * page_size < 2^31. */
+int mosaic_paged_step(const int32_t* lengths, const int32_t* add, int32_t* block_table, int64_t table_stride,
+                      const int32_t* free_pages, const int32_t* free_count, int64_t requests, int64_t width,
+                      int64_t pages, int64_t tokens, int64_t page_size, int32_t* starts, int32_t* lengths_out,
+                      int32_t* seq_lens, int32_t* positions, int32_t* slots, int32_t* count_out, void* stream);
+
+/* Shortens requests to keep[r] tokens (0 releases one; more than it holds
+ * changes nothing) and pushes the pages behind them, the last request's last
+ * page first: the inverse of a step.  `pages` is the stack's capacity; the
+ * tables are left as they are.  lengths_out and count_out may not overlap the
+ * inputs (free_pages is updated in place). */
+int mosaic_paged_trim(const int32_t* lengths, const int32_t* keep, const int32_t* block_table, int64_t table_stride,
+                      int32_t* free_pages, const int32_t* free_count, int64_t requests, int64_t width, int64_t pages,
+                      int64_t page_size, int32_t* lengths_out, int32_t* count_out, void* stream);
+
+/* Writes the step's keys and values k, v [tokens, kv_heads, head_dim] bf16
+ * (strides in elements, multiples of 8; 16-byte aligned; head_dim 64, 128 or
+ * 256) into the cache.  A block and head's scale is the least power of two 2^e,
+ * e >= -126, with its largest finite magnitude at most 448 2^e; codes are
+ * e4m3(x / 2^e), nearest even, infinities to +-448, NaN kept.  Where a block
+ * held tokens before, its scale only grows, and the old codes are rounded to
+ * the new one; the rest of a block that begins in this call is zeroed, bytes
+ * behind the last token of an older one are left.  Blocks that take new tokens
+ * must belong to one request. */
+int mosaic_paged_kv_write(const uint16_t* k, const uint16_t* v, int64_t k_token_stride, int64_t k_head_stride,
+                          int64_t v_token_stride, int64_t v_head_stride, int64_t tokens, uint8_t* codes,
+                          uint8_t* scales, int64_t pages, int64_t blocks, int64_t kv_heads, int64_t head_dim,
+                          const int32_t* block_table, int64_t table_stride, int64_t width, const int32_t* starts,
+                          const int32_t* seq_lens, int64_t requests, void* stream);
+
+/* Causal attention of the batch's rows over the cache: row t of request r is
+ * position seq_lens[r] - (starts[r + 1] - starts[r]) + t and sees the keys up to
+ * itself, with window > 0 only the last `window` of them.  q [tokens, q_heads,
+ * head_dim] bf16 (strides in elements, multiples of 8; 16-byte aligned), query
+ * head h reads key head h / (q_heads / kv_heads); sink [q_heads] f32 or NULL adds
+ * exp(sink) to the softmax denominator.  out [tokens, q_heads, head_dim] bf16,
+ * contiguous; rows without a key, and rows behind the last request, are zero.
+ * max_new: the most rows of any request, or 0 if not known (it only sizes the
+ * launch). */
+size_t mosaic_paged_attention_workspace_bytes(int64_t tokens, int64_t requests, int64_t q_heads, int64_t kv_heads,
+                                              int64_t head_dim);
+int mosaic_paged_attention(const uint16_t* q, int64_t q_token_stride, int64_t q_head_stride, int64_t tokens,
+                           int64_t q_heads, const uint8_t* codes, const uint8_t* scales, int64_t pages, int64_t blocks,
+                           int64_t kv_heads, int64_t head_dim, const int32_t* block_table, int64_t table_stride,
+                           int64_t width, const int32_t* starts, const int32_t* seq_lens, int64_t requests,
+                           const float* sink, int64_t window, int64_t max_new, float softmax_scale, uint16_t* out,
+                           void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

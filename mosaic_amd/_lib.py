@@ -82,6 +82,13 @@ SIGNATURES: dict[str, tuple] = {
     "mosaic_mla_sparse_decode_bf16": (c_int, [P, P, P, P, P, I64, I64, I64, I64, I64, I64, F, P, c_size_t, P]),
     "mosaic_dsa_kv_write": (c_int, [P, P, I64, I64, I64, I64, P, P, P, P, P]),
     "mosaic_dsa_decode_indices": (c_int, [P, I64, I64, P, I64, I64, I64, P, P]),
+    "mosaic_paged_step": (c_int, [P, P, P, I64, P, P, I64, I64, I64, I64, I64, P, P, P, P, P, P, P]),
+    "mosaic_paged_trim": (c_int, [P, P, P, I64, P, P, I64, I64, I64, I64, P, P, P]),
+    "mosaic_paged_kv_write": (c_int, [P, P, I64, I64, I64, I64, I64, P, P, I64, I64, I64, I64, P, I64, I64, P, P, I64,
+                                      P]),
+    "mosaic_paged_attention_workspace_bytes": (c_size_t, [I64, I64, I64, I64, I64]),
+    "mosaic_paged_attention": (c_int, [P, I64, I64, I64, I64, P, P, I64, I64, I64, I64, P, I64, I64, P, P, I64, P, I64,
+                                       I64, F, P, P, c_size_t, P]),
     "mosaic_rmsnorm_act_quant": (c_int, [P, P, F, I64, I64, P, P, P, c_int, P]),
     "mosaic_swiglu_act_quant": (c_int, [P, P, I64, I64, F, P, P, P]),
     "mosaic_routed_reduce": (c_int, [P, P, P, P, I64, I64, I64, I64, P]),

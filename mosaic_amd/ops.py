@@ -991,3 +991,222 @@ def dsa_decode_indices(pos: torch.Tensor, window: int, cidx: torch.Tensor | None
               _stream())
     return out
 
+
+
+# -------------------------------------------------------- paged KV cache ----
+PAGED_BLOCK = 64  # tokens that share a scale
+
+
+def _index(t: torch.Tensor, name: str, shape: tuple, device) -> torch.Tensor:
+    """An int32 index array as it is (no copy: the caller's own buffers are read and updated)."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor, got {type(t).__name__}")
+    if t.dtype != torch.int32:
+        raise ValueError(f"{name}: expected int32, got {t.dtype}")
+    if t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {list(shape)}, got {list(t.shape)}")
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, expected {device}")
+    return t
+
+
+def _table(t: torch.Tensor, rows: int, device) -> torch.Tensor:
+    """A block table [R, B] int32; its rows may be the first B entries of longer ones."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"block_table must be a torch.Tensor, got {type(t).__name__}")
+    if t.dtype != torch.int32 or t.dim() != 2 or t.shape[0] != rows or t.shape[1] < 1 or \
+            t.stride(1) != 1 or (rows > 1 and t.stride(0) < t.shape[1]):
+        raise ValueError(f"block_table must be [{rows}, B] int32 with unit inner stride, got {list(t.shape)} {t.dtype} "
+                         f"strides {t.stride()}")
+    if t.device != device:
+        raise ValueError(f"block_table is on {t.device}, expected {device}")
+    return t
+
+
+def _row_stride(t: torch.Tensor) -> int:
+    return max(t.stride(0), t.shape[1])
+
+
+def _call_on(device: torch.device, name: str, *args) -> None:
+    """``_lib.call`` on the current stream of `device`, whichever device is current."""
+    if device.index == torch.cuda.current_device():
+        _lib.call(name, *args, _stream())
+        return
+    with torch.cuda.device(device):
+        _lib.call(name, *args, _stream())
+
+
+@dataclass
+class PagedStep:
+    """What one step of a paged batch reads: token rows ``starts[r] .. starts[r + 1]``
+    of request r, its tokens with them ``seq_lens[r]`` (0: not placed), the
+    ``positions`` and cache ``slots`` of the token rows (-1: none), and the pool's
+    state after the step, ``lengths`` and ``free_count``.  All are int32 views of
+    one buffer, so a serving loop makes one (``PagedStep.empty``) and reuses it."""
+
+    starts: torch.Tensor
+    lengths: torch.Tensor
+    free_count: torch.Tensor
+    seq_lens: torch.Tensor
+    positions: torch.Tensor
+    slots: torch.Tensor
+
+    @classmethod
+    def empty(cls, requests: int, tokens: int, device) -> "PagedStep":
+        buf = torch.empty(3 * requests + 2 + 2 * tokens, dtype=torch.int32, device=device)
+        return cls(*buf.split((requests + 1, requests, 1, requests, tokens, tokens)))
+
+
+def paged_step(lengths: torch.Tensor, new: torch.Tensor, block_table: torch.Tensor, tokens: int, page_size: int,
+               free_pages: torch.Tensor | None = None, free_count: torch.Tensor | None = None,
+               out: PagedStep | None = None) -> PagedStep:
+    """Block tables and slot map of one step, on the GPU: request r holds
+    ``lengths[r]`` tokens and adds ``new[r]``, whose rows follow each other in a
+    buffer of ``tokens`` rows.  New pages are popped from the stack ``free_pages``
+    (``free_count`` [1] of them) into ``block_table`` [R, B], which is updated in
+    place; without ``free_pages`` the tables hold the pages already.  Requests
+    are placed in order; one whose rows, table or pages do not suffice is not
+    placed: its length stays, its ``seq_lens`` is 0, its rows have no slot.  The
+    inputs other than the table are left as they are (``out`` may not share
+    their memory): commit a step by copying ``lengths`` and ``free_count``."""
+    if not isinstance(lengths, torch.Tensor) or not lengths.is_cuda or lengths.dim() != 1:
+        raise ValueError("lengths must be a GPU tensor [R] (mosaic_amd has no CPU path)")
+    dev, r = lengths.device, lengths.shape[0]
+    lengths, new = _index(lengths, "lengths", (r,), dev), _index(new, "new", (r,), dev)
+    block_table = _table(block_table, r, dev)
+    if (free_pages is None) != (free_count is None):
+        raise ValueError("free_pages goes with free_count")
+    pages = 0
+    if free_pages is not None:
+        pages = free_pages.numel()
+        free_pages, free_count = _index(free_pages, "free_pages", (pages,), dev), _index(free_count, "free_count", (1,), dev)
+    tokens = int(tokens)
+    if out is None:
+        if tokens < 0:
+            raise ValueError(f"tokens {tokens}")
+        out = PagedStep.empty(r, tokens, dev)
+    else:
+        for name, n in (("starts", r + 1), ("lengths", r), ("free_count", 1), ("seq_lens", r), ("positions", tokens),
+                        ("slots", tokens)):
+            _index(getattr(out, name), "out." + name, (n,), dev)
+    _call_on(dev, "mosaic_paged_step", _ptr(lengths), _ptr(new), _ptr(block_table), _row_stride(block_table),
+             _ptr(free_pages), _ptr(free_count), r, block_table.shape[1], pages, tokens, int(page_size),
+             _ptr(out.starts), _ptr(out.lengths), _ptr(out.seq_lens), _ptr(out.positions), _ptr(out.slots),
+             _ptr(out.free_count))
+    return out
+
+
+def paged_trim(lengths: torch.Tensor, keep: torch.Tensor, block_table: torch.Tensor, page_size: int,
+               free_pages: torch.Tensor, free_count: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """Shorten requests to ``keep[r]`` tokens (0 releases one; more than it holds
+    changes nothing) and push the pages behind them onto ``free_pages``, in
+    place: the inverse of ``paged_step``.  -> (lengths [R], free_count [1])."""
+    if not isinstance(lengths, torch.Tensor) or not lengths.is_cuda or lengths.dim() != 1:
+        raise ValueError("lengths must be a GPU tensor [R] (mosaic_amd has no CPU path)")
+    dev, r = lengths.device, lengths.shape[0]
+    lengths, keep = _index(lengths, "lengths", (r,), dev), _index(keep, "keep", (r,), dev)
+    block_table = _table(block_table, r, dev)
+    if not isinstance(free_pages, torch.Tensor):
+        raise TypeError(f"free_pages must be a torch.Tensor, got {type(free_pages).__name__}")
+    pages = free_pages.numel()
+    free_pages, free_count = _index(free_pages, "free_pages", (pages,), dev), _index(free_count, "free_count", (1,), dev)
+    kept, count = torch.empty(r + 1, dtype=torch.int32, device=dev).split((r, 1))
+    _call_on(dev, "mosaic_paged_trim", _ptr(lengths), _ptr(keep), _ptr(block_table), _row_stride(block_table),
+             _ptr(free_pages), _ptr(free_count), r, block_table.shape[1], pages, int(page_size), _ptr(kept),
+             _ptr(count))
+    return kept, count
+
+
+def _paged_cache(codes: torch.Tensor, scales: torch.Tensor, device) -> tuple:
+    """codes [P, NB, Hkv, 2, 64 D] and scales [P, NB, Hkv, 2], read and written in place -> (P, NB, Hkv, D)."""
+    for t, name, dtypes in ((codes, "codes", (torch.uint8, torch.float8_e4m3fn)),
+                            (scales, "scales", (torch.uint8, torch.float8_e8m0fnu))):
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name} must be a torch.Tensor, got {type(t).__name__}")
+        if t.dtype not in dtypes or not t.is_contiguous() or t.device != device:
+            raise ValueError(f"{name} must be contiguous bytes on {device}, got {t.dtype} on {t.device}")
+    if codes.dim() != 5 or codes.shape[3] != 2 or codes.shape[4] % PAGED_BLOCK or scales.shape != codes.shape[:4]:
+        raise ValueError(f"codes must be [P, NB, Hkv, 2, 64 D] and scales [P, NB, Hkv, 2], got {list(codes.shape)} and "
+                         f"{list(scales.shape)}")
+    p, nb, hkv = codes.shape[:3]
+    return p, nb, hkv, codes.shape[4] // PAGED_BLOCK
+
+
+def _paged_rows(t: torch.Tensor, name: str) -> torch.Tensor:
+    """bf16 [T, H, D] read through its strides, or a copy where 16 bytes cannot be read at a time."""
+    if _on_device(t, name).dtype != torch.bfloat16:
+        raise ValueError(f"{name}: expected bfloat16, got {t.dtype}")
+    if t.dim() != 3:
+        raise ValueError(f"{name} must be [T, H, D], got {list(t.shape)}")
+    if t.stride(2) != 1 or t.stride(0) % 8 or t.stride(1) % 8 or t.data_ptr() % 16:
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def paged_kv_write(k: torch.Tensor, v: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
+                   block_table: torch.Tensor, starts: torch.Tensor, seq_lens: torch.Tensor) -> None:
+    """Write a step's keys and values k, v [T, Hkv, D] bf16 (D = 64, 128 or 256)
+    into the paged cache, 8 bits a value: ``codes`` [P, NB, Hkv, 2, 64 D] e4m3 and
+    ``scales`` [P, NB, Hkv, 2] e8m0, one scale a block of 64 tokens and head,
+    2^e with the largest magnitude at most 448 2^e.  ``starts`` and ``seq_lens`` as in
+    ``PagedStep``.  A block that held tokens before keeps its scale or moves to a
+    larger one; the rest of a block that begins here is zeroed."""
+    k, v = _paged_rows(k, "k"), _paged_rows(v, "v")
+    dev = k.device
+    if v.device != dev or v.shape != k.shape:
+        raise ValueError(f"k {list(k.shape)} on {dev} and v {list(v.shape)} on {v.device} do not agree")
+    p, nb, hkv, d = _paged_cache(codes, scales, dev)
+    t = k.shape[0]
+    if tuple(k.shape[1:]) != (hkv, d):
+        raise ValueError(f"k {list(k.shape)} does not match a cache of {hkv} heads of {d}")
+    if not isinstance(seq_lens, torch.Tensor) or seq_lens.dim() != 1:
+        raise ValueError("seq_lens must be a tensor [R]")
+    r = seq_lens.shape[0]
+    starts, seq_lens = _index(starts, "starts", (r + 1,), dev), _index(seq_lens, "seq_lens", (r,), dev)
+    block_table = _table(block_table, r, dev)
+    _call_on(dev, "mosaic_paged_kv_write", _ptr(k), _ptr(v), k.stride(0), k.stride(1), v.stride(0), v.stride(1), t,
+             _ptr(codes), _ptr(scales), p, nb, hkv, d, _ptr(block_table), _row_stride(block_table),
+             block_table.shape[1], _ptr(starts), _ptr(seq_lens), r)
+
+
+def paged_attention(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, block_table: torch.Tensor,
+                    starts: torch.Tensor, seq_lens: torch.Tensor, softmax_scale: float,
+                    sink: torch.Tensor | None = None, window: int = 0, max_new: int | None = None,
+                    out: torch.Tensor | None = None, workspace: MoEWorkspace | None = None) -> torch.Tensor:
+    """Causal grouped-query attention of a ragged batch over the paged 8-bit
+    cache: q [T, Hq, D] bf16 (its strides are followed), Hq a multiple of the
+    cache's Hkv -> o [T, Hq, D] bf16.  Row t of request r is position
+    seq_lens[r] - (its rows) + t and sees the tokens up to itself, with ``window``
+    only that many of them; ``sink`` [Hq] f32 adds exp(sink) to the denominator.
+    Decode steps, drafts, pieces of prompts and whole prompts may share a call.
+    Rows without a key and rows behind the last request are zero.  ``max_new``:
+    the most rows of any request where the caller knows it (it only sizes the
+    launches).  A ``workspace`` serves one call at a time: calls on other
+    streams, and graphs that may replay at once, need one each."""
+    q = _paged_rows(q, "q")
+    dev = q.device
+    p, nb, hkv, d = _paged_cache(codes, scales, dev)
+    t, hq, dq = q.shape
+    if dq != d or hq % hkv or hq == 0:
+        raise ValueError(f"q {list(q.shape)} does not match a cache of {hkv} heads of {d}")
+    if not isinstance(seq_lens, torch.Tensor) or seq_lens.dim() != 1:
+        raise ValueError("seq_lens must be a tensor [R]")
+    r = seq_lens.shape[0]
+    starts, seq_lens = _index(starts, "starts", (r + 1,), dev), _index(seq_lens, "seq_lens", (r,), dev)
+    block_table = _table(block_table, r, dev)
+    if sink is not None:
+        sink = _f32(sink, "sink")
+        if tuple(sink.shape) != (hq,) or sink.device != dev:
+            raise ValueError(f"sink must be [{hq}] on {dev}, got {list(sink.shape)} on {sink.device}")
+    if max_new is not None and max_new < 1:
+        raise ValueError(f"max_new {max_new}")
+    if out is None:
+        out = torch.empty(t, hq, d, dtype=torch.bfloat16, device=dev)
+    elif out.shape != q.shape or out.dtype != torch.bfloat16 or not out.is_contiguous() or out.device != dev:
+        raise ValueError(f"out must be a contiguous bf16 {list(q.shape)} on {dev}")
+    nbytes = _lib.lib().mosaic_paged_attention_workspace_bytes(t, r, hq, hkv, d)
+    ws = _workspace(workspace, nbytes, dev)
+    _call_on(dev, "mosaic_paged_attention", _ptr(q), q.stride(0), q.stride(1), t, hq, _ptr(codes), _ptr(scales), p, nb,
+             hkv, d, _ptr(block_table), _row_stride(block_table), block_table.shape[1], _ptr(starts), _ptr(seq_lens),
+             r, _ptr(sink), int(window), int(max_new or 0), float(softmax_scale), _ptr(out), _ptr(ws), ws.numel())
+    return out

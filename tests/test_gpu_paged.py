@@ -1,0 +1,526 @@
+"""The paged 8-bit KV cache on the GPU against the oracle: tables, slots, codes and scales bit for bit,
+attention within the bound that ``oracle.paged.attention`` derives, and the parts together."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import codecs as C
+from oracle import paged as P
+
+pytestmark = pytest.mark.gpu
+
+
+def _i32(a, dev):
+    return torch.from_numpy(np.ascontiguousarray(a, dtype=np.int32)).to(dev)
+
+
+def _bf16(rng, *shape):
+    return C.round_bf16(rng.standard_normal(shape).astype(np.float32))
+
+
+def _pool(rng, lengths, after, page, spare):
+    """Tables [R, B] that hold `lengths` tokens of requests that grow to `after`, and a stack of free pages."""
+    held = [-(-max(int(x), 0) // page) for x in lengths]
+    fresh = sum(-(-max(int(b), 0) // page) for b in after) - sum(held)
+    total = sum(held) + max(fresh, 0) + spare
+    ids = rng.permutation(total).astype(np.int32)
+    width = max(1, max(-(-max(int(b), 0) // page) for b in after)) + 1
+    table = rng.integers(-5, 5, (len(lengths), width)).astype(np.int32)  # behind the last page: anything
+    at = 0
+    for i, n in enumerate(held):
+        table[i, :n] = ids[at:at + n]
+        at += n
+    free = np.full(total, -9, np.int32)
+    free[:total - at] = ids[at:]
+    return table, free, total - at, total
+
+
+# ----------------------------------------------------------- step, trim ----
+@pytest.mark.parametrize("r,most,n,page,pad,dry,allocate", [
+    (1, 1, 1, 64, 0, False, True), (1, 0, 1, 64, 3, False, True), (16, 500, 1, 64, 0, False, True),
+    (7, 300, 200, 128, 5, False, True), (64, 1000, 3, 192, 0, True, True), (1024, 200, 2, 64, 1, False, True),
+    (1025, 200, 5, 64, 0, True, True), (2500, 90, 20, 64, 77, False, True), (3, 5000, 4000, 64, 0, False, True),
+    (300, 64, 130, 64, 0, True, True), (40, 400, 60, 256, 2, False, False), (5, 70, 0, 64, 4, False, True)])
+def test_step(dev, r, most, n, page, pad, dry, allocate):
+    from mosaic_amd import ops
+    rng = np.random.default_rng(r + most + n)
+    lengths = rng.integers(0, most + 1, r).astype(np.int32)
+    new = rng.integers(0, n + 1, r).astype(np.int32)
+    if r > 4:
+        lengths[3], new[2] = -5, -2  # read as nothing
+    after = np.maximum(lengths, 0) + np.maximum(new, 0)
+    table, free, count, total = _pool(rng, lengths if allocate else after, after, page, 3)
+    if dry:
+        count = count // 2
+    tokens = int(np.maximum(new, 0).sum()) + pad
+    t = _i32(table, dev)
+    args = dict(free_pages=_i32(free, dev), free_count=_i32([count], dev)) if allocate else {}
+    lt, nt = _i32(lengths, dev), _i32(new, dev)
+    s = ops.paged_step(lt, nt, t, tokens, page, **args)
+    want = P.step(lengths, new, table, tokens, page, free if allocate else None, count if allocate else 0)
+    for name, x in want.items():
+        np.testing.assert_array_equal(getattr(s, name).cpu().numpy(), x, err_msg=name)
+    np.testing.assert_array_equal(t.cpu().numpy(), table)
+    np.testing.assert_array_equal(lt.cpu().numpy(), lengths)
+    if dry:
+        assert (want["seq_lens"] == 0).any() and int(want["free_count"][0]) >= 0
+
+
+def test_step_rows_and_tables_that_do_not_suffice(dev):
+    from mosaic_amd import ops
+    rng = np.random.default_rng(5)
+    lengths, new = np.array([10, 64, 100, 0, 3], np.int32), np.array([5, 200, 2 ** 30, 7, 1], np.int32)
+    table, free, count, _ = _pool(rng, lengths, lengths + 70, 64, 9)
+    for tokens in (0, 4, 5, 300, 205 + (1 << 20)):
+        tb = table.copy()
+        t = _i32(tb, dev)
+        s = ops.paged_step(_i32(lengths, dev), _i32(new, dev), t, tokens, 64, _i32(free, dev), _i32([count], dev))
+        want = P.step(lengths, new, tb, tokens, 64, free, count)
+        for name, x in want.items():
+            np.testing.assert_array_equal(getattr(s, name).cpu().numpy(), x, err_msg=f"{tokens} {name}")
+        np.testing.assert_array_equal(t.cpu().numpy(), tb)
+
+
+def test_step_without_requests(dev):
+    from mosaic_amd import ops
+    s = ops.paged_step(_i32([], dev), _i32([], dev), torch.zeros(0, 3, dtype=torch.int32, device=dev), 5, 64,
+                       _i32([4, 2], dev), _i32([2], dev))
+    assert s.starts.tolist() == [0] and s.positions.tolist() == [-1] * 5 and s.free_count.tolist() == [2]
+
+
+@pytest.mark.parametrize("r,most,page", [(1, 500, 64), (33, 2000, 64), (1024, 300, 128), (1030, 700, 64), (2100, 64, 64)])
+def test_trim(dev, r, most, page):
+    from mosaic_amd import ops
+    rng = np.random.default_rng(r)
+    lengths = rng.integers(0, most + 1, r).astype(np.int32)
+    keep = np.where(rng.random(r) < 0.3, 0, lengths - rng.integers(-3, 70, r)).astype(np.int32)
+    table, free, count, total = _pool(rng, lengths, lengths, page, 4)
+    t, f = _i32(table, dev), _i32(free, dev)
+    kept, left = ops.paged_trim(_i32(lengths, dev), _i32(keep, dev), t, page, f, _i32([count], dev))
+    want, n = P.trim(lengths, keep, table, page, free, count)
+    np.testing.assert_array_equal(kept.cpu().numpy(), want)
+    np.testing.assert_array_equal(f.cpu().numpy(), free)
+    assert left.tolist() == [n]
+    np.testing.assert_array_equal(t.cpu().numpy(), table)
+
+
+def test_trim_onto_a_full_stack_writes_nothing_past_it(dev):
+    from mosaic_amd import ops
+    f = torch.arange(6, dtype=torch.int32, device=dev)
+    guard = f.clone()
+    kept, left = ops.paged_trim(_i32([300], dev), _i32([0], dev), _i32([[1, 2, 3, 4, 5]], dev), 64, f[:3], _i32([2], dev))
+    assert kept.tolist() == [0] and left.tolist() == [3]
+    assert f.tolist() == guard[:2].tolist() + [5] + guard[3:].tolist()
+
+
+# ---------------------------------------------------------------- write ----
+def _cache(rng, total, nb, hkv, d):
+    codes = rng.integers(0, 256, (total, nb, hkv, 2, 64 * d)).astype(np.uint8)
+    codes[(codes & 0x7F) == 0x7F] = 0x30
+    return codes, rng.integers(118, 124, (total, nb, hkv, 2)).astype(np.uint8)
+
+
+def _batch(rng, held, new, page, spare=2):
+    held, new = np.array(held), np.array(new)
+    seq = held + new
+    table, _, _, total = _pool(rng, seq, seq, page, spare)
+    starts = np.concatenate([[0], np.cumsum(new)]).astype(np.int32)
+    return table, total, starts, seq.astype(np.int32)
+
+
+def _same_codes(got, want):
+    """Equal bytes; a NaN's sign is free."""
+    nan = (want & 0x7F) == 0x7F
+    np.testing.assert_array_equal((got & 0x7F)[nan], want[nan] & 0x7F)
+    np.testing.assert_array_equal(got[~nan], want[~nan])
+
+
+@pytest.mark.parametrize("hkv,d,page,held,new", [
+    (1, 64, 64, [0], [1]), (2, 128, 64, [0, 5, 63, 64, 65], [1, 1, 1, 1, 1]), (8, 128, 64, [0, 10], [64, 128]),
+    (3, 64, 128, [7, 0, 100, 130], [150, 3, 28, 0]), (2, 256, 192, [190, 1], [5, 300]), (4, 128, 256, [0], [700]),
+    (5, 64, 64, list(range(0, 300)), [2] * 300)])
+def test_write(dev, hkv, d, page, held, new):
+    from mosaic_amd import ops
+    rng = np.random.default_rng(hkv * d + len(held))
+    table, total, starts, seq = _batch(rng, held, new, page)
+    codes, scales = _cache(rng, total, page // 64, hkv, d)
+    t = int(starts[-1]) + 3  # rows behind the last request are not read
+    k, v = _bf16(rng, t, hkv, d) * 2.0 ** rng.integers(-8, 5, (t, 1, 1)), _bf16(rng, t, hkv, d) * 0.01
+    k[int(starts[-1]):] = np.nan
+    kv = torch.from_numpy(np.concatenate([k, v], 1).astype(np.float32)).to(dev).to(torch.bfloat16)
+    ct, st = torch.from_numpy(codes).to(dev), torch.from_numpy(scales).to(dev)
+    ops.paged_kv_write(kv[:, :hkv], kv[:, hkv:], ct, st, _i32(table, dev), _i32(starts, dev), _i32(seq, dev))
+    x = kv.double().cpu().numpy()  # the oracle gets the bf16 values that the call gets
+    P.write(x[:, :hkv], x[:, hkv:], codes, scales, table, starts, seq)
+    np.testing.assert_array_equal(st.cpu().numpy(), scales)
+    _same_codes(ct.cpu().numpy(), codes)
+
+
+def test_write_extremes(dev):
+    """Zeros, bf16's smallest and largest, infinities and NaN; a scale that grows by one and by many powers."""
+    from mosaic_amd import ops
+    rng = np.random.default_rng(8)
+    hkv, d = 6, 64
+    table, total, starts, seq = _batch(rng, [0, 20, 40], [70, 9, 2], 64)
+    codes, scales = _cache(rng, total, 1, hkv, d)
+    t = int(starts[-1])
+    k = _bf16(rng, t, hkv, d).astype(np.float64)
+    k[:, 0] = 0.0
+    k[:, 1] *= 2.0 ** -130
+    k[:, 2] *= 2.0 ** 120
+    k[::3, 3, ::5], k[1::3, 3, ::7], k[2::3, 3, ::9] = np.inf, -np.inf, np.nan
+    k[:, 4] = np.inf
+    k[:, 5, :] = 448.0 * 2.0 ** 3
+    k = C.round_bf16(k.astype(np.float32)).astype(np.float64)
+    scales[:, :, 0] = 1
+    codes[:, 0, 3, 1, ::11] = 0xFF
+    x = torch.from_numpy(k.astype(np.float32)).to(dev).to(torch.bfloat16)
+    ct, st = torch.from_numpy(codes).to(dev), torch.from_numpy(scales).to(dev)
+    ops.paged_kv_write(x, x, ct, st, _i32(table, dev), _i32(starts, dev), _i32(seq, dev))
+    P.write(k, k, codes, scales, table, starts, seq)
+    np.testing.assert_array_equal(st.cpu().numpy(), scales)
+    _same_codes(ct.cpu().numpy(), codes)
+
+
+def test_write_skips_what_is_not_placed(dev):
+    """Requests with seq_lens 0, pages outside the pool and starts outside the rows change nothing."""
+    from mosaic_amd import ops
+    rng = np.random.default_rng(9)
+    codes, scales = _cache(rng, 4, 1, 2, 64)
+    x = torch.from_numpy(_bf16(rng, 30, 2, 64)).to(dev).to(torch.bfloat16)
+    ct, st = torch.from_numpy(codes).to(dev), torch.from_numpy(scales).to(dev)
+    table = _i32([[0, 1], [4, -1], [2, 3], [3, 3]], dev)
+    ops.paged_kv_write(x, x, ct, st, table, _i32([0, 10, 20, 20, 20], dev), _i32([0, 10, 50, 7], dev))
+    ops.paged_kv_write(x, x, ct, st, table, _i32([30, 40, 100, 2 ** 31 - 1, 2 ** 31 - 1], dev), _i32([64, 128, 128, 64], dev))
+    np.testing.assert_array_equal(ct.cpu().numpy(), codes)
+    np.testing.assert_array_equal(st.cpu().numpy(), scales)
+
+
+# ------------------------------------------------------------ attention ----
+def _attention_case(dev, rng, hq, hkv, d, page, held, new, window=0, sink=False, pad=0, max_new=None, codes=None,
+                    change=None, scale=None):
+    from mosaic_amd import ops
+    table, total, starts, seq = _batch(rng, held, new, page)
+    c, s = _cache(rng, total, page // 64, hkv, d)
+    if change is not None:
+        change(c, s, table, seq, starts)
+    t = int(starts[-1]) + pad
+    q = _bf16(rng, t, hq, d)
+    snk = rng.standard_normal(hq).astype(np.float32) if sink else None
+    scale = d ** -0.5 if scale is None else scale
+    qt = torch.from_numpy(q).to(dev).to(torch.bfloat16)
+    out = torch.full((t, hq, d), float("nan"), dtype=torch.bfloat16, device=dev)
+    got = ops.paged_attention(qt, torch.from_numpy(c).to(dev), torch.from_numpy(s).to(dev), _i32(table, dev),
+                              _i32(starts, dev), _i32(seq, dev), scale,
+                              sink=None if snk is None else torch.from_numpy(snk).to(dev), window=window,
+                              max_new=max_new, out=out)
+    assert got.data_ptr() == out.data_ptr()
+    want, tol = P.attention(q.astype(np.float64), c, s, table, starts, seq, scale, snk, window)
+    o = out.float().cpu().numpy().astype(np.float64)
+    np.testing.assert_array_equal(np.isnan(o), np.isnan(want))
+    bad = ~(np.abs(o - want) <= tol) & ~np.isnan(want)
+    assert not bad.any(), f"{bad.sum()} values off, worst {np.nanmax(np.abs(o - want) / np.maximum(tol, 1e-30))} of the bound"
+
+
+@pytest.mark.parametrize("hq,hkv,d,page,held,new,window,sink", [
+    (1, 1, 64, 64, [0], [1], 0, False),                       # one token alone
+    (8, 1, 128, 64, [0, 1, 62, 63, 64, 500], [1] * 6, 0, False),
+    (64, 8, 128, 64, [516], [1], 0, True),
+    (16, 2, 128, 128, [2000, 3, 127, 128], [1] * 4, 0, True),
+    (14, 2, 64, 64, [300, 20], [1, 1], 100, False),           # seven heads a key head
+    (6, 6, 64, 192, [700, 10, 0], [1, 1, 1], 64, True),       # a key head each
+    (32, 2, 256, 64, [130, 999], [1, 1], 0, False),           # sixteen heads a key head
+    (40, 2, 128, 64, [150], [1], 0, False),                   # twenty: two tiles
+    (16, 2, 128, 64, [100, 0, 37, 700], [4, 2, 0, 3], 0, True),      # drafts, a resting request
+    (16, 2, 128, 64, [100, 0, 37], [4, 2, 3], 5, False),
+    (8, 2, 64, 64, [0], [200], 0, False),                     # a prompt
+    (8, 2, 128, 64, [0, 70, 5], [130, 1, 65], 0, True),       # pieces of prompts and a decode step
+    (8, 1, 256, 128, [60], [150], 33, True),
+    (4, 4, 64, 64, [0, 200], [129, 70], 128, False)])
+def test_attention(dev, hq, hkv, d, page, held, new, window, sink):
+    rng = np.random.default_rng(hq + d + len(held) + window)
+    _attention_case(dev, rng, hq, hkv, d, page, held, new, window, sink, max_new=max(new))
+    _attention_case(dev, rng, hq, hkv, d, page, held, new, window, sink, pad=3)
+
+
+def test_attention_long_context(dev):
+    """Few rows over a long axis: cut among all workgroups and joined."""
+    rng = np.random.default_rng(11)
+    _attention_case(dev, rng, 8, 1, 128, 64, [40000], [1], sink=True)
+    _attention_case(dev, rng, 4, 2, 64, 256, [30001, 5, 12345], [1, 2, 1])
+
+
+def test_attention_many_short_requests(dev):
+    rng = np.random.default_rng(12)
+    held = rng.integers(0, 200, 700)
+    _attention_case(dev, rng, 4, 1, 64, 64, held, rng.integers(0, 3, 700), pad=2)
+
+
+def test_attention_scale_bytes(dev):
+    """The least and largest scales that the writer makes of bf16 values near its range's ends, mixed in one row."""
+    def change(c, s, table, seq, starts):
+        s[..., 0] = 100  # small keys: flat scores
+        s[table[0, 0], :, :, 1] = 20
+        s[table[0, 1], :, :, 1] = 200
+        s[table[0, 2], :, :, 1] = 127
+    _attention_case(dev, np.random.default_rng(13), 8, 2, 128, 64, [180], [3], change=change)
+
+
+def test_attention_does_not_read_behind_a_request(dev):
+    """NaN codes behind the last token and before a window, NaN scales and pages of no pool that no row sees."""
+    def change(c, s, table, seq, starts):
+        for i in range(len(seq)):
+            at_k, at_v = P.block_maps(64)
+            lo = max(0, int(seq[i]) - 1 - 99 - 64)
+            for b in range(-(-int(seq[i]) // 64)):
+                for tok in range(64):
+                    p = 64 * b + tok
+                    if p >= seq[i] or p < int(seq[i]) - (int(starts[i + 1]) - int(starts[i])) - 99:
+                        c[table[i, b], 0, :, 0][:, at_k[tok]] = 0x7F
+                        c[table[i, b], 0, :, 1][:, at_v[tok]] = 0xFF
+            for b in range(lo // 64):
+                s[table[i, b]] = 255
+                table[i, b] = [-1, 1 << 30][b % 2]
+    _attention_case(dev, np.random.default_rng(14), 8, 2, 64, 64, [300, 10, 700, 500], [1, 1, 3, 100], window=100,
+                    sink=True, change=change)
+
+
+def test_attention_nan_reaches_only_rows_that_see_it(dev):
+    """NaN keys and values of tokens in the middle of the new ones: earlier rows stay numbers, each dim by itself."""
+    def change(c, s, table, seq, starts):
+        at_k, at_v = P.block_maps(64)
+        c[table[0, 0], 0, 0, 1, at_v[40, 5:7]] = 0x7F
+        c[table[0, 0], 0, 1, 0, at_k[50, 9]] = 0xFF
+        s[table[0, 2], 0, 1, 1] = 255
+        s[table[1, 0], 0, 0, 0] = 255
+    _attention_case(dev, np.random.default_rng(15), 4, 2, 64, 64, [30, 20], [150, 30], change=change)
+
+
+def test_attention_pages_outside_the_pool_hold_no_keys(dev):
+    def change(c, s, table, seq, starts):
+        table[0, 1], table[1, 0], table[2, :] = -1, c.shape[0], -7
+    _attention_case(dev, np.random.default_rng(16), 8, 2, 128, 64, [200, 30, 100], [2, 40, 1], sink=True, change=change)
+
+
+def test_attention_unplaced_requests_give_zeros(dev):
+    from mosaic_amd import ops
+    rng = np.random.default_rng(17)
+    c, s = _cache(rng, 3, 1, 1, 64)
+    q = torch.from_numpy(_bf16(rng, 6, 2, 64)).to(dev).to(torch.bfloat16)
+    out = torch.full_like(q, float("nan"))
+    o = ops.paged_attention(q, torch.from_numpy(c).to(dev), torch.from_numpy(s).to(dev), _i32([[0], [1], [2]], dev),
+                            _i32([0, 2, 3, 4], dev), _i32([0, 9, 0], dev), 0.125,
+                            sink=torch.zeros(2, device=dev), out=out)
+    assert not o[[0, 1, 3, 4, 5]].any() and o[2].abs().max() > 0
+
+
+def test_attention_starts_outside_the_rows(dev):
+    """Starts that pass the rows are cut: no row outside is read or written."""
+    from mosaic_amd import ops
+    rng = np.random.default_rng(18)
+    c, s = _cache(rng, 3, 1, 1, 64)
+    q = torch.from_numpy(_bf16(rng, 8, 2, 64)).to(dev).to(torch.bfloat16)
+    buf = torch.full((10, 2, 64), 7.0, dtype=torch.bfloat16, device=dev)
+    for starts in ([0, 100, 200, 300], [-5, 3, 1, 2 ** 31 - 1], [9, 9, 9, 9]):
+        ops.paged_attention(q, torch.from_numpy(c).to(dev), torch.from_numpy(s).to(dev), _i32([[0], [1], [2]], dev),
+                            _i32(starts, dev), _i32([64, 9, 2 ** 31 - 1], dev), 0.125, out=buf[1:9])
+        assert (buf[0] == 7).all() and (buf[9] == 7).all()
+
+
+def test_attention_strided_and_unaligned_q(dev):
+    from mosaic_amd import ops
+    rng = np.random.default_rng(19)
+    table, total, starts, seq = _batch(rng, [70, 3], [1, 5], 64)
+    c, s = (torch.from_numpy(x).to(dev) for x in _cache(rng, total, 1, 2, 64))
+    qkv = torch.from_numpy(_bf16(rng, 6, 8 * 64 + 8)).to(dev).to(torch.bfloat16)
+    args = (c, s, _i32(table, dev), _i32(starts, dev), _i32(seq, dev), 0.125)
+    for q in (qkv[:, :256].view(6, 4, 64), qkv[:, 8:264].view(6, 4, 64), qkv[:, 3:259].view(6, 4, 64),
+              qkv[:, :512].view(6, 8, 64)[:, ::2], qkv[:, :256].reshape(6, 64, 4).transpose(1, 2)):
+        assert torch.equal(ops.paged_attention(q, *args), ops.paged_attention(q.clone(memory_format=torch.contiguous_format), *args))
+    wide = torch.full((2, 50), -1, dtype=torch.int32, device=dev)
+    wide[:, 3:3 + table.shape[1]] = _i32(table, dev)
+    cut = wide[:, 3:3 + table.shape[1]]
+    q = qkv[:, :256].view(6, 4, 64)
+    assert torch.equal(ops.paged_attention(q, c, s, cut, *args[3:]), ops.paged_attention(q, *args))
+
+
+def test_attention_repeats_its_bits(dev):
+    from mosaic_amd import ops
+    rng = np.random.default_rng(20)
+    table, total, starts, seq = _batch(rng, [3000, 3, 900], [1, 2, 300], 64)
+    c, s = (torch.from_numpy(x).to(dev) for x in _cache(rng, total, 1, 2, 128))
+    q = torch.from_numpy(_bf16(rng, 303, 8, 128)).to(dev).to(torch.bfloat16)
+    ws = ops.MoEWorkspace()
+    args = (q, c, s, _i32(table, dev), _i32(starts, dev), _i32(seq, dev), 0.1)
+    first = ops.paged_attention(*args)
+    for _ in range(5):
+        assert torch.equal(ops.paged_attention(*args, workspace=ws), first)
+
+
+def test_codes_past_32_bits(dev):
+    """A pool of more than 4 GiB: its last pages are written and read at their own place."""
+    from mosaic_amd import ops
+    rng = np.random.default_rng(21)
+    hkv, d = 8, 256
+    pages = (1 << 32) // (hkv * 2 * 64 * d) + 40
+    codes = torch.zeros(pages, 1, hkv, 2, 64 * d, dtype=torch.uint8, device=dev)
+    scales = torch.full((pages, 1, hkv, 2), 127, dtype=torch.uint8, device=dev)
+    k, v = (torch.from_numpy(_bf16(rng, 90, hkv, d)).to(dev).to(torch.bfloat16) for _ in range(2))
+    q = torch.from_numpy(_bf16(rng, 90, hkv, d)).to(dev).to(torch.bfloat16)
+    outs = []
+    for ids in ([pages - 1, pages - 30], [0, 1]):
+        table = _i32([ids], dev)
+        st, sq = _i32([0, 90], dev), _i32([90], dev)
+        ops.paged_kv_write(k, v, codes, scales, table, st, sq)
+        outs.append(ops.paged_attention(q, codes, scales, table, st, sq, d ** -0.5))
+    assert torch.equal(*outs)
+    assert torch.equal(codes[pages - 1], codes[0]) and torch.equal(codes[pages - 30], codes[1])
+    assert not codes[2:pages - 30].any() and not codes[pages - 29:pages - 1].any()
+
+
+# ------------------------------------------------------------- together ----
+class _Model:
+    """The cache's parts together, in the oracle."""
+
+    def __init__(self, pages, hkv, d, r, most, page, layers):
+        self.page = page
+        self.codes = np.zeros((layers, pages, page // 64, hkv, 2, 64 * d), np.uint8)
+        self.scales = np.full((layers, pages, page // 64, hkv, 2), 127, np.uint8)
+        self.table = np.full((r, -(-most // page)), -1, np.int32)
+        self.free, self.count = np.arange(pages - 1, -1, -1).astype(np.int32), pages
+        self.lengths = np.zeros(r, np.int32)
+
+    def step(self, new, tokens):
+        s = P.step(self.lengths, new, self.table, tokens, self.page, self.free, self.count)
+        self.lengths, self.count = s["lengths"], int(s["free_count"][0])
+        return s
+
+    def trim(self, keep):
+        self.lengths, self.count = P.trim(self.lengths, keep, self.table, self.page, self.free, self.count)
+
+
+def test_serving_run(dev):
+    """Prompts, decode steps, drafts that are rejected, requests that end and begin, a pool that runs dry."""
+    from mosaic_amd.kernels.paged import PagedKVCache
+    rng = np.random.default_rng(22)
+    r, hq, hkv, d, page, layers, pages, most = 5, 8, 2, 64, 64, 2, 14, 400
+    cache = PagedKVCache(pages, hkv, d, r, most, page, layers, dev)
+    model = _Model(pages, hkv, d, r, most, page, layers)
+    sink = rng.standard_normal(hq).astype(np.float32)
+    plan = [([130, 5, 0, 64, 1], None), ([1, 1, 70, 1, 1], None), ([4, 4, 4, 4, 4], [133, 8, 73, 66, 4]),
+            ([1, 1, 1, 1, 1], [0, 9, 74, 67, 0]), ([200, 1, 1, 1, 33], None), ([1, 300, 1, 400, 90], None),
+            ([1, 1, 1, 1, 1], [0, 0, 0, 0, 0]), ([63, 64, 65, 1, 2], None)]
+    refused = 0
+    for new, keep in plan:
+        tokens = sum(new) + 2
+        s = cache.step(_i32(new, dev), tokens)
+        w = model.step(np.array(new), tokens)
+        for name, x in w.items():
+            np.testing.assert_array_equal(getattr(s, name).cpu().numpy(), x, err_msg=name)
+        refused += int(((w["seq_lens"] == 0) & (np.array(new) > 0)).sum())
+        for layer in range(layers):
+            q, k, v = _bf16(rng, tokens, hq, d), _bf16(rng, tokens, hkv, d), _bf16(rng, tokens, hkv, d)
+            t = [torch.from_numpy(x).to(dev).to(torch.bfloat16) for x in (q, k, v)]
+            o = cache.update(s, *t, 0.125, sink=torch.from_numpy(sink).to(dev), layer=layer,
+                             max_new=max(new)).float().cpu().numpy()
+            P.write(k.astype(np.float64), v.astype(np.float64), model.codes[layer], model.scales[layer], model.table,
+                    w["starts"], w["seq_lens"])
+            np.testing.assert_array_equal(cache.scales[layer].cpu().numpy(), model.scales[layer])
+            np.testing.assert_array_equal(cache.codes[layer].cpu().numpy(), model.codes[layer])
+            want, tol = P.attention(q.astype(np.float64), model.codes[layer], model.scales[layer], model.table,
+                                    w["starts"], w["seq_lens"], 0.125, sink)
+            assert np.all(np.abs(o - want) <= tol)
+        if keep is not None:
+            cache.trim(_i32(keep, dev))
+            model.trim(np.array(keep))
+        np.testing.assert_array_equal(cache.lengths.cpu().numpy(), model.lengths)
+        assert cache.free_count.tolist() == [model.count]
+        np.testing.assert_array_equal(cache.free_pages.cpu().numpy()[:model.count], model.free[:model.count])
+    assert refused
+
+
+def test_decode_steps_in_a_graph(dev):
+    """A captured decode step (tables, write, attention, commit), replayed beside the same steps run eagerly."""
+    from mosaic_amd import ops
+    from mosaic_amd.kernels.paged import PagedKVCache
+    rng = np.random.default_rng(23)
+    r, hq, hkv, d = 3, 8, 2, 64
+    caches = [PagedKVCache(20, hkv, d, r, 300, device=dev) for _ in range(2)]
+    first = _i32([60, 1, 127], dev)
+    prompt = [torch.from_numpy(_bf16(rng, 188, h, d)).to(dev).to(torch.bfloat16) for h in (hq, hkv, hkv)]
+    for c in caches:
+        c.update(c.step(first, 188), *prompt, 0.125)
+    one = torch.ones(r, dtype=torch.int32, device=dev)
+    x = [torch.zeros(r, h, d, dtype=torch.bfloat16, device=dev) for h in (hq, hkv, hkv)]
+    ws = ops.MoEWorkspace()
+    out = ops.PagedStep.empty(r, r, dev)
+    state = [t.clone() for t in (caches[0].codes, caches[0].scales, caches[0].block_table, caches[0].lengths, caches[0].free_count)]
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):  # the library and workspace are warm
+        caches[0].update(caches[0].step(one, r, out), *x, 0.125, max_new=1, workspace=ws)
+    stream.synchronize()
+    for t, was in zip((caches[0].codes, caches[0].scales, caches[0].block_table, caches[0].lengths, caches[0].free_count), state):
+        t.copy_(was)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        o = caches[0].update(caches[0].step(one, r, out), *x, 0.125, max_new=1, workspace=ws)
+    for i in range(8):
+        for t in x:
+            t.copy_(torch.from_numpy(_bf16(rng, *t.shape)).to(dev))
+        graph.replay()
+        torch.cuda.synchronize()
+        want = caches[1].update(caches[1].step(one, r), *x, 0.125, max_new=1)
+        assert torch.equal(o, want), i
+        assert torch.equal(caches[0].codes, caches[1].codes) and torch.equal(caches[0].lengths, caches[1].lengths)
+        assert torch.equal(caches[0].block_table, caches[1].block_table)
+
+
+def test_other_stream(dev):
+    """The operators run on torch's current stream, behind what was put there before."""
+    from mosaic_amd import ops
+    rng = np.random.default_rng(24)
+    table, total, starts, seq = _batch(rng, [500, 70], [1, 1], 64)
+    c, s = (torch.from_numpy(x).to(dev) for x in _cache(rng, total, 1, 2, 128))
+    args = (c, s, _i32(table, dev), _i32(starts, dev), _i32(seq, dev), 0.1)
+    q = torch.from_numpy(_bf16(rng, 2, 8, 128)).to(dev).to(torch.bfloat16)
+    want = ops.paged_attention(q, *args)
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        late = torch.zeros_like(q)
+        for _ in range(50):
+            late = late + 0  # work in front
+        late.copy_(q)
+        got = ops.paged_attention(late, *args)
+    stream.synchronize()
+    assert torch.equal(got, want)
+
+
+def test_refusals_of_the_wrappers(dev):
+    from mosaic_amd import ops
+    z = lambda *s, dt=torch.int32: torch.zeros(*s, dtype=dt, device=dev)  # noqa: E731
+    q, codes, scales = z(2, 4, 64, dt=torch.bfloat16), z(3, 1, 2, 2, 64 * 64, dt=torch.uint8), z(3, 1, 2, 2, dt=torch.uint8)
+    ok = dict(q=q, codes=codes, scales=scales, block_table=z(2, 3), starts=z(3), seq_lens=z(2), softmax_scale=1.0)
+    ops.paged_attention(**ok)
+    for kw in (dict(q=q.float()), dict(q=q[0]), dict(q=z(2, 3, 64, dt=torch.bfloat16)), dict(codes=codes[..., ::2]),
+               dict(codes=codes.int()), dict(scales=scales[:2]), dict(block_table=z(2, 3).long()), dict(starts=z(2)),
+               dict(seq_lens=z(2).long()), dict(seq_lens=z(4)[::2]), dict(sink=z(3, dt=torch.float32)), dict(window=-1),
+               dict(max_new=0), dict(out=q[:1]), dict(block_table=z(3, 3)), dict(starts=z(3).cpu())):
+        with pytest.raises((ValueError, TypeError)):
+            ops.paged_attention(**{**ok, **kw})
+    k = z(2, 2, 64, dt=torch.bfloat16)
+    ok = dict(k=k, v=k, codes=codes, scales=scales, block_table=z(2, 3), starts=z(3), seq_lens=z(2))
+    ops.paged_kv_write(**ok)
+    for kw in (dict(k=k.half()), dict(v=k[:1]), dict(k=z(2, 1, 64, dt=torch.bfloat16)), dict(codes=codes[:, :, :1])):
+        with pytest.raises((ValueError, TypeError)):
+            ops.paged_kv_write(**{**ok, **kw})
+    ok = dict(lengths=z(2), new=z(2), block_table=z(2, 3), tokens=2, page_size=64, free_pages=z(3), free_count=z(1))
+    ops.paged_step(**ok)
+    same = z(2)
+    for kw in (dict(tokens=-1), dict(page_size=16), dict(new=z(3)), dict(free_count=None), dict(lengths=z(2).float()),
+               dict(out=ops.PagedStep.empty(2, 3, dev)), dict(lengths=same, out=ops.PagedStep(z(3), same, z(1), z(2), z(2), z(2)))):
+        with pytest.raises((ValueError, TypeError)):
+            ops.paged_step(**{**ok, **kw})
