@@ -86,7 +86,7 @@ SIGNATURES: dict[str, tuple] = {
     "mosaic_paged_trim": (c_int, [P, P, P, I64, P, P, I64, I64, I64, I64, P, P, P]),
     "mosaic_paged_kv_write": (c_int, [P, P, I64, I64, I64, I64, I64, P, P, I64, I64, I64, I64, P, I64, I64, P, P, I64,
                                       P]),
-    "mosaic_paged_attention_workspace_bytes": (c_size_t, [I64, I64, I64, I64, I64]),
+    "mosaic_paged_attention_workspace_bytes": (c_size_t, [I64, I64, I64, I64, I64, I64, I64, I64]),
     "mosaic_paged_attention": (c_int, [P, I64, I64, I64, I64, P, P, I64, I64, I64, I64, P, I64, I64, P, P, I64, P, I64,
                                        I64, F, P, P, c_size_t, P]),
     "mosaic_rmsnorm_act_quant": (c_int, [P, P, F, I64, I64, P, P, P, c_int, P]),

@@ -20,7 +20,10 @@
 // (q, c) then holds four tokens of row c, which are its own operand of
 // O^T = V^T P^T; the cache stores the values in that order, so neither keys,
 // values nor probabilities pass through LDS or between lanes.
+#include <limits.h>
+
 #include <cmath>
+#include <type_traits>
 
 #include "common.h"
 #include "../../include/mosaic_amd.h"
@@ -41,14 +44,20 @@ struct AttnArgs {
   uint16_t* out;
   float* part_o;   // [2 kGroups][16][D], unnormalized
   float* part_ml;  // [2 kGroups][2][16]
-  int32_t* info;   // [0]: tiles; from [4]: [tiles][Hkv][4]: first row, rows, the runs of its first and last piece
+  int32_t* info;   // [0]: tiles; from [8]: [tiles][Hkv][8]: first row, rows, pieces, slots of the first and second
+                   // piece, from one piece's slot to the next's (a slot: partial sums of 16 rows)
+  float *tile_o, *tile_ml;  // the same of the many-row kernel, where it cuts tiles
+  int32_t* tile_info;
   int64_t q_tok, q_head, stride;
-  int r, tokens, hq, hkv, group, width, pages, nb, window, tiles;
-  float scale;  // softmax scale times log2(e)
+  int r, tokens, hq, hkv, group, width, pages, nb, window;
+  int rows_max;    // requests of more rows are the many-row kernel's
+  bool zero_rows;  // the many-row kernel clears what lies behind the last request
+  float scale;     // |softmax scale| log2(e)
+  float sign;      // of the softmax scale
 };
 
 struct Request {
-  int s0, n, held, first, blocks, tiles;  // first: the first block that any row sees
+  int s0, n, held, first, blocks, rows;  // first: the first block that any row sees
 };
 
 __device__ __forceinline__ Request request_of(const AttnArgs& a, int r) {
@@ -60,10 +69,15 @@ __device__ __forceinline__ Request request_of(const AttnArgs& a, int r) {
     x.held = seq - x.n;
     x.first = a.window && x.held + 1 > a.window ? (x.held + 1 - a.window) / kBlock : 0;
     x.blocks = max((seq + kBlock - 1) / kBlock - x.first, 1);  // a tile without tokens still writes its zeros
-    x.tiles = (x.n * a.group + kRows - 1) / kRows;
+    x.rows = x.n * a.group;
   }
   return x;
 }
+// row tiles of 16 of a request that is not left to the many-row kernel
+__device__ __forceinline__ int few_tiles(const AttnArgs& a, const Request& x) {
+  return x.rows > a.rows_max ? 0 : (x.rows + kRows - 1) / kRows;
+}
+__device__ __forceinline__ bool many_rows(const AttnArgs& a, const Request& x) { return x.rows > a.rows_max; }
 
 __device__ __forceinline__ float lane4_max(float x) {  // over the four lanes of a column
   const auto r16 = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -101,13 +115,14 @@ __global__ void __launch_bounds__(64 * NW) paged_attn_rows_kernel(const AttnArgs
   __shared__ uint32_t sums[NW], sums_t[NW], s_unit;
   __shared__ int s_req, s_tile;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, q = lane >> 4, c = lane & 15;
+  const float scale = a.scale * a.sign;
 
   // every workgroup counts the units of all requests; then the one that holds its run's first unit
   uint32_t total = 0, tiles_all = 0;
   for (int base = 0; base < a.r; base += 64 * NW) {
     const Request x = request_of(a, base + tid);
-    const uint32_t n = (uint32_t)(x.tiles * a.hkv) * (uint32_t)x.blocks;
-    const uint32_t incl = wave_incl_scan_u32(n), tinc = wave_incl_scan_u32((uint32_t)x.tiles);
+    const uint32_t t = (uint32_t)few_tiles(a, x), n = t * (uint32_t)a.hkv * (uint32_t)x.blocks;
+    const uint32_t incl = wave_incl_scan_u32(n), tinc = wave_incl_scan_u32(t);
     if (lane == 63) {
       sums[wave] = incl;
       sums_t[wave] = tinc;
@@ -134,8 +149,8 @@ __global__ void __launch_bounds__(64 * NW) paged_attn_rows_kernel(const AttnArgs
     uint32_t tiles = 0;
     for (int base = 0; base < a.r; base += 64 * NW) {
       const Request x = request_of(a, base + tid);
-      const uint32_t n = (uint32_t)(x.tiles * a.hkv) * (uint32_t)x.blocks;
-      const uint32_t incl = wave_incl_scan_u32(n), tinc = wave_incl_scan_u32((uint32_t)x.tiles);
+      const uint32_t t = (uint32_t)few_tiles(a, x), n = t * (uint32_t)a.hkv * (uint32_t)x.blocks;
+      const uint32_t incl = wave_incl_scan_u32(n), tinc = wave_incl_scan_u32(t);
       if (lane == 63) {
         sums[wave] = incl;
         sums_t[wave] = tinc;
@@ -154,7 +169,7 @@ __global__ void __launch_bounds__(64 * NW) paged_attn_rows_kernel(const AttnArgs
       if (u0 >= at && u0 - at < n) {
         s_req = base + tid;
         s_unit = at;
-        s_tile = (int)(t_at + tinc) - x.tiles;
+        s_tile = (int)(t_at + tinc - t);
       }
       __syncthreads();
       if (seen > u0) break;
@@ -164,19 +179,21 @@ __global__ void __launch_bounds__(64 * NW) paged_attn_rows_kernel(const AttnArgs
   int r = s_req, tile0 = s_tile;
   uint32_t req0 = s_unit;
   Request x = request_of(a, r);
-    for (uint32_t u = u0; u < u1;) {
-    while (u - req0 >= (uint32_t)(x.tiles * a.hkv) * (uint32_t)x.blocks) {
-      req0 += (uint32_t)(x.tiles * a.hkv) * (uint32_t)x.blocks;
-      tile0 += x.tiles;
+  uint32_t tiles = (uint32_t)few_tiles(a, x);
+  for (uint32_t u = u0; u < u1;) {
+    while (u - req0 >= tiles * (uint32_t)a.hkv * (uint32_t)x.blocks) {
+      req0 += tiles * (uint32_t)a.hkv * (uint32_t)x.blocks;
+      tile0 += (int)tiles;
       x = request_of(a, ++r);
+      tiles = (uint32_t)few_tiles(a, x);
     }
     // unit -> (head, tile, block), blocks fastest
     const uint32_t in = u - req0, ht = in / (uint32_t)x.blocks;
     const int b_from = (int)(in % (uint32_t)x.blocks), b_to = (int)min((uint32_t)x.blocks, (uint32_t)b_from + (u1 - u));
-    const int h = (int)(ht / (uint32_t)x.tiles), tile = (int)(ht % (uint32_t)x.tiles);
+    const int h = (int)(ht / tiles), tile = (int)(ht % tiles);
     const uint32_t tile_u0 = u - b_from;
     u += b_to - b_from;
-    const int row0 = tile * kRows, rows = min(kRows, x.n * a.group - row0);
+    const int row0 = tile * kRows, rows = min(kRows, x.rows - row0);
     const int row = row0 + min(c, rows - 1);
     const int tok = row / a.group, head = h * a.group + row % a.group;
     const int pos = x.held + tok;
@@ -234,7 +251,7 @@ __global__ void __launch_bounds__(64 * NW) paged_attn_rows_kernel(const AttnArgs
       for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          float v = s[t][i] * a.scale;
+          float v = s[t][i] * scale;
           if (edge) {
             const int p = t0 + 16 * t + 4 * q + i;
             v = ke == 255u ? NAN : v;
@@ -338,11 +355,13 @@ __global__ void __launch_bounds__(64 * NW) paged_attn_rows_kernel(const AttnArgs
     // a piece that begins inside its tile is its run's first, one that only ends inside is its last
     const int slot = 2 * (int)blockIdx.x + (b_from == 0 ? 1 : 0);
     if (b_from == 0 && tid == 0) {  // the join's list: this tile's rows and the runs that hold it
-      int32_t* t = a.info + 4 + ((int64_t)(tile0 + tile) * a.hkv + h) * 4;
+      int32_t* t = a.info + 8 + ((int64_t)(tile0 + tile) * a.hkv + h) * 8;
       t[0] = (x.s0 + row0 / a.group) * a.group + row0 % a.group;
       t[1] = rows;
-      t[2] = (int)blockIdx.x;
-      t[3] = (int)((tile_u0 + x.blocks - 1) / share);
+      t[2] = (int)((tile_u0 + x.blocks - 1) / share - blockIdx.x) + 1;
+      t[3] = slot;
+      t[4] = slot + 1;
+      t[5] = 2;
     }
     float inv = 0.f;
     if (whole) {
@@ -379,43 +398,43 @@ __global__ void __launch_bounds__(64 * NW) paged_attn_rows_kernel(const AttnArgs
 // Adds up the pieces of a tile that was cut: one workgroup a row, its 256
 // threads as groups of D / 4 lanes (four dims each) that take the pieces in turn.
 template <int D>
-__global__ void __launch_bounds__(256) paged_attn_join_kernel(const AttnArgs a) {
+__global__ void __launch_bounds__(256) paged_attn_join_kernel(const AttnArgs a, const int32_t* __restrict__ info) {
   constexpr int LANES = D / 4, SG = 256 / LANES;
   __shared__ f32x4_t so[SG][LANES];
-  __shared__ float red[4][2];
-  const int tile = blockIdx.x, h = blockIdx.y, c = blockIdx.z, tid = threadIdx.x;
-  if (tile >= a.info[0]) return;
-  const int32_t* t = a.info + 4 + ((int64_t)tile * a.hkv + h) * 4;
-  const int w0 = t[2], w1 = t[3];
-  if (w0 == w1 || c >= t[1]) return;
-  const int row = t[0] + c, head = h * a.group + row % a.group;
-  auto slot = [&](int i) { return (int64_t)(i == 0 ? 2 * w0 + 1 : 2 * (w0 + i)); };
-  const int n = w1 - w0 + 1;
+  __shared__ float red[4], ls[SG];
+  const int tile = blockIdx.x, h = blockIdx.y, i = blockIdx.z, tid = threadIdx.x;
+  if (tile >= info[0]) return;
+  const int32_t* t = info + 8 + ((int64_t)tile * a.hkv + h) * 8;
+  const int n = t[2];
+  if (n == 1 || i >= t[1]) return;
+  const int row = t[0] + i, head = h * a.group + row % a.group;
+  const int64_t first = (int64_t)(t[3] + i / 16), second = (int64_t)(t[4] + i / 16), step = t[5];
+  const int c = i % 16;
+  auto slot = [&](int p) { return p == 0 ? first : second + step * (p - 1); };
   float m = -INFINITY;
-  for (int i = tid; i < n; i += 256) m = fmaxf(m, a.part_ml[slot(i) * 32 + c]);
+  for (int p = tid; p < n; p += 256) m = fmaxf(m, a.part_ml[slot(p) * 32 + c]);
   m = wave_max_f32(m);
-  if ((tid & 63) == 0) red[tid >> 6][0] = m;
+  if ((tid & 63) == 0) red[tid >> 6] = m;
   __syncthreads();
-  m = fmaxf(fmaxf(red[0][0], red[1][0]), fmaxf(red[2][0], red[3][0]));
+  m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
   const float ref = m == -INFINITY ? 0.f : m;
   const int g = tid / LANES, d = tid % LANES;
   f32x4_t o = {0.f, 0.f, 0.f, 0.f};
   float l = 0.f;
 #pragma unroll 8
-  for (int i = g; i < n; i += SG) {
-    const float f = __builtin_amdgcn_exp2f(a.part_ml[slot(i) * 32 + c] - ref);
-    l += f * a.part_ml[slot(i) * 32 + 16 + c];
-    o += *reinterpret_cast<const f32x4_t*>(a.part_o + (slot(i) * 16 + c) * D + 4 * d) * f;
+  for (int p = g; p < n; p += SG) {
+    const float f = __builtin_amdgcn_exp2f(a.part_ml[slot(p) * 32 + c] - ref);
+    l += f * a.part_ml[slot(p) * 32 + 16 + c];
+    o += *reinterpret_cast<const f32x4_t*>(a.part_o + (slot(p) * 16 + c) * D + 4 * d) * f;
   }
-  __shared__ float ls[SG];
   so[g][d] = o;
   if (d == 0) ls[g] = l;
   __syncthreads();
   if (g) return;
 #pragma unroll
-  for (int i = 1; i < SG; ++i) {
-    o += so[i][d];
-    l += ls[i];
+  for (int p = 1; p < SG; ++p) {
+    o += so[p][d];
+    l += ls[p];
   }
   const float s_ = a.sink ? a.sink[head] * kLog2e : -INFINITY;
   const float inv = m == -INFINITY ? l : 1.f / (l + __builtin_amdgcn_exp2f(s_ - ref));
@@ -425,31 +444,425 @@ __global__ void __launch_bounds__(256) paged_attn_join_kernel(const AttnArgs a) 
   *reinterpret_cast<uint2*>(a.out + ((int64_t)(row / a.group) * a.hq + head) * D + 4 * d) = pk;
 }
 
-struct Sizes {
-  int64_t tiles, info, part_o, part_ml, total;
-};
+// ---------------------------------------------------------- many rows ----
+// Requests of many rows (prompts and their pieces): a workgroup owns 32 NW rows of
+// a key head, 32 a wave, and its waves share the blocks, which are copied
+// straight into LDS, two ahead.
+//
+//   scores   S^T = K Q^T in bf16 (32 x 32 x 16), codes converted with their scale as
+//            they come out of LDS.  (Codes as they are, against q in two e4m3 parts on
+//            the fp8 unit, were slower: a prompt of 4096 tokens, 64 heads of 128, 376
+//            against 323 us; and its sums are not as exact as fp32.)
+//   values   O^T = V^T P^T in bf16 (32 x 32 x 16), codes converted with their
+//            scale as they come out of LDS; lane (h, c) holds tokens
+//            8 i + 4 h + .. of row c, which are its operand.
+// The running reference of the exponentials follows the maximum only when it
+// has grown by more than 2^8: p is then at most 2^8, with the same relative
+// rounding, and O is seldom scaled.
 
-Sizes sizes(int64_t tokens, int64_t requests, int64_t hq, int64_t hkv, int64_t d) {
-  Sizes s;
-  s.tiles = tokens * (hq / hkv) / kRows + (requests < tokens ? requests : tokens);
-  s.part_o = (int64_t)2 * kGroups * kRows * d * 4;
-  s.part_ml = (int64_t)2 * kGroups * 2 * kRows * 4;
-  s.info = 16 + s.tiles * hkv * 16;
-  s.total = s.part_o + s.part_ml + s.info;
-  return s;
+typedef __attribute__((ext_vector_type(16))) float f32x16_t;
+
+constexpr float kLazy = 8.f;  // log2
+
+__device__ __forceinline__ float half_max(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float half_sum(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ void lds_copy16(const void* g, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(__builtin_amdgcn_readfirstlane(lds)),
+               "v"(g) : "memory", "m0");
+}
+// own copies but the last N are in LDS, own LDS reads are done, and so are the other waves'
+template <int N>
+__device__ __forceinline__ void stage_ready() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
 
 template <int D, int NW>
-int launch(const AttnArgs& a, int rows, hipStream_t st) {
-  MOSAIC_LAUNCH((paged_attn_rows_kernel<D, NW>), dim3(kGroups), dim3(64 * NW), 0, st, a);
-  MOSAIC_LAUNCH_CHECK("paged_attention");
-  MOSAIC_LAUNCH(paged_attn_join_kernel<D>, dim3((unsigned)a.tiles, (unsigned)a.hkv, (unsigned)rows), dim3(256), 0, st, a);
-  MOSAIC_RETURN_LAUNCH("paged_attention");
+__global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) paged_attn_tile_kernel(const AttnArgs a) {
+  constexpr int DG = D / 64, DQ = D / 32, ROWS = 32 * NW, STAGE = 2 * kBlock * D;
+  constexpr int STAGES = 3, CPW = STAGE / 1024 / NW;  // copies of 1 KB a wave and block
+  static_assert(CPW >= 1, "every wave copies");
+  __shared__ __attribute__((aligned(16))) uint8_t buf[STAGES * STAGE];
+  __shared__ uint32_t sums[NW];
+  __shared__ int s_req, s_tile;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int hl = lane >> 5, c = lane & 31, c16 = lane & 15, up = (lane >> 4) & 1;
+
+  if (a.zero_rows && blockIdx.x == 0 && blockIdx.y == 0) {
+    const int64_t from = a.r ? min(max(a.starts[a.r], 0), a.tokens) : 0, per = (int64_t)a.hq * D;
+    for (int64_t i = from * per + 8 * tid; i < a.tokens * per; i += 8 * 64 * NW)
+      *reinterpret_cast<u32x4_t*>(a.out + i) = u32x4_t{0u, 0u, 0u, 0u};
+  }
+  // the request and tile: key heads fastest (a head's workgroups meet in one XCD's
+  // L2 where there are eight), the last tiles, which see most, first
+  const int h = blockIdx.x % a.hkv;
+  uint32_t total = 0;
+  for (int base = 0; base < a.r; base += 64 * NW) {
+    const Request x = request_of(a, base + tid);
+    const uint32_t n = many_rows(a, x) ? (uint32_t)((x.rows + ROWS - 1) / ROWS) : 0u;
+    const uint32_t incl = wave_incl_scan_u32(n);
+    if (lane == 63) sums[wave] = incl;
+    __syncthreads();
+    for (int w = 0; w < NW; ++w) total += sums[w];
+    __syncthreads();
+  }
+  if (blockIdx.x == 0 && blockIdx.y == 0 && tid == 0 && gridDim.y > 1) a.tile_info[0] = (int32_t)total;
+  const uint32_t idx = blockIdx.x / a.hkv;
+  if (idx >= total) return;
+  const uint32_t want = total - 1 - idx;
+  {
+    uint32_t seen = 0;
+    for (int base = 0; base < a.r; base += 64 * NW) {
+      const Request x = request_of(a, base + tid);
+      const uint32_t n = many_rows(a, x) ? (uint32_t)((x.rows + ROWS - 1) / ROWS) : 0u;
+      const uint32_t incl = wave_incl_scan_u32(n);
+      if (lane == 63) sums[wave] = incl;
+      __syncthreads();
+      uint32_t at = seen + incl - n;
+      for (int w = 0; w < NW; ++w) {
+        if (w < wave) at += sums[w];
+        seen += sums[w];
+      }
+      if (want >= at && want - at < n) {
+        s_req = base + tid;
+        s_tile = (int)(want - at);
+      }
+      __syncthreads();
+      if (seen > want) break;
+    }
+  }
+  __syncthreads();
+  const int r = __builtin_amdgcn_readfirstlane(s_req), tile = __builtin_amdgcn_readfirstlane(s_tile);
+  const Request x = request_of(a, r);
+  const int row0 = tile * ROWS, rows = min(ROWS, x.rows - row0);
+  const int limit = a.width * a.nb * kBlock;
+  // blocks that the tile sees, and this workgroup's share of them
+  const int tile_hi = min(max(x.held + (row0 + rows - 1) / a.group + 1, 0), limit);
+  const int tile_lo = a.window ? max(x.held + row0 / a.group + 1 - a.window, 0) : 0;
+  const int first = tile_lo / kBlock, all_blocks = max((tile_hi + kBlock - 1) / kBlock - first, 0);
+  const int b0 = __builtin_amdgcn_readfirstlane(first + (int)((int64_t)all_blocks * blockIdx.y / gridDim.y));
+  const int nblk = __builtin_amdgcn_readfirstlane(first + (int)((int64_t)all_blocks * (blockIdx.y + 1) / gridDim.y)) - b0;
+
+  // the wave's rows, and between which tokens all and any of them see
+  const int wrow0 = row0 + 32 * wave, wrows = min(32, rows - 32 * wave);  // wrows <= 0: a wave without rows
+  const int row = wrow0 + min(c, max(wrows, 1) - 1);
+  const int safe = min(row, x.rows - 1);
+  const int tok = safe / a.group, head = h * a.group + safe % a.group, pos = x.held + tok;
+  const int row_hi = min(max(pos + 1, 0), limit), row_lo = a.window ? max(pos + 1 - a.window, 0) : 0;
+  const int tok_a = wrow0 / a.group, tok_b = (wrow0 + max(wrows, 1) - 1) / a.group;
+  const int any_hi = wrows > 0 ? max(x.held + tok_b + 1, 0) : 0, all_hi = max(x.held + tok_a + 1, 0);
+  const int any_lo = a.window ? max(x.held + tok_a + 1 - a.window, 0) : 0;
+  const int all_lo = a.window ? max(x.held + tok_b + 1 - a.window, 0) : 0;
+
+  // q: 32 dims of a row for each 64, in the order of the keys' bytes
+  bf16x8_t qf[DG][4];
+  {
+    const uint16_t* qrow = a.q + (int64_t)(x.s0 + tok) * a.q_tok + (int64_t)head * a.q_head + 32 * hl;
+    const uint32_t flip = a.sign < 0.f ? 0x80008000u : 0u;
+#pragma unroll
+    for (int g = 0; g < DG; ++g)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        u32x4_t w = *reinterpret_cast<const u32x4_t*>(qrow + 64 * g + 8 * i);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) w[k] ^= flip;
+        qf[g][i] = __builtin_bit_cast(bf16x8_t, w);
+      }
+  }
+
+  // pages and scales of the 64 blocks from `meta` on, one a lane
+  const int32_t* trow = a.table + (int64_t)r * a.stride;
+  int meta = 0, pages_ = -1;
+  uint32_t scales_ = 0u;
+  auto load_meta = [&](int at) {
+    meta = at;
+    const int blk = b0 + at + lane;
+    pages_ = -1;
+    scales_ = 0u;
+    if (at + lane < nblk) {
+      pages_ = trow[blk / a.nb];
+      if (pages_ < 0 || pages_ >= a.pages) pages_ = -1;
+      const int64_t unit = ((int64_t)max(pages_, 0) * a.nb + blk % a.nb) * a.hkv + h;
+      scales_ = *reinterpret_cast<const uint16_t*>(a.scales + unit * 2);
+    }
+  };
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)buf;
+  // block j into its stage; -> its scales, or ~0 where it has no page
+  auto issue = [&](int j) -> uint32_t {
+    if (j >= nblk) return 0u;
+    if (j - meta >= 64) load_meta(j);
+    const int page = __builtin_amdgcn_readlane(pages_, j - meta);
+    const uint32_t sc = (uint32_t)__builtin_amdgcn_readlane((int)scales_, j - meta);
+    const int64_t unit = ((int64_t)max(page, 0) * a.nb + (b0 + j) % a.nb) * a.hkv + h;
+    const uint8_t* src = a.codes + unit * STAGE + (wave * CPW) * 1024 + lane * 16;
+    const uint32_t dst = lds0 + (uint32_t)(j % STAGES) * STAGE + (uint32_t)(wave * CPW) * 1024;
+#pragma unroll
+    for (int i = 0; i < CPW; ++i) lds_copy16(src + i * 1024, dst + i * 1024);
+    return page < 0 ? ~0u : sc;
+  };
+  load_meta(0);
+  uint32_t sc_cur = issue(0), sc_next = issue(1);
+
+  float m = -INFINITY, ref = 0.f, l = 0.f;  // m: of the raw scores; ref: what the exponents are taken against
+  f32x16_t o[DQ];
+#pragma unroll
+  for (int j = 0; j < DQ; ++j)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[j][i] = 0.f;
+
+  // one block; EDGE: some row does not see it whole, it has no page, or a scale is no number
+  auto block = [&](auto edge, const uint8_t* kb, int t0, bool good, uint32_t ke, uint32_t ve) __attribute__((always_inline)) {
+    constexpr bool EDGE = decltype(edge)::value;
+    f32x16_t s[2];
+    const float ks = e8m0_f32(ke);
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[t][i] = 0.f;
+#pragma unroll
+      for (int g = 0; g < DG; ++g) {
+        const u32x4_t* p = reinterpret_cast<const u32x4_t*>(kb + (((2 * t + up) * DG + g) * 64 + 2 * hl * 16 + c16) * 16);
+        const u32x4_t k0 = p[0], k1 = p[16];
+        s[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(to_bf16(k0[0], k0[1], ks), qf[g][0], s[t], 0, 0, 0);
+        s[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(to_bf16(k0[2], k0[3], ks), qf[g][1], s[t], 0, 0, 0);
+        s[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(to_bf16(k1[0], k1[1], ks), qf[g][2], s[t], 0, 0, 0);
+        s[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(to_bf16(k1[2], k1[3], ks), qf[g][3], s[t], 0, 0, 0);
+      }
+    }
+    const int hi = good ? row_hi : 0;
+    if constexpr (EDGE) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int p = t0 + 32 * t + 8 * (i >> 2) + 4 * hl + (i & 3);
+          const float v = ke == 255u ? NAN : s[t][i];
+          s[t][i] = p < hi && p >= row_lo ? v : -INFINITY;
+        }
+    }
+    float bm = fmaxf(s[0][0], s[1][0]);
+#pragma unroll
+    for (int i = 1; i < 16; ++i) bm = fmaxf(fmaxf(bm, s[0][i]), s[1][i]);
+    bm = half_max(bm);
+    const bool fresh = m == -INFINITY && bm != -INFINITY;  // the first keys of a row set its reference
+    m = fmaxf(m, bm);
+    const float mn = m == -INFINITY ? 0.f : m * a.scale;
+    if (__ballot(mn - ref > kLazy || fresh)) {
+      const float to = (mn - ref > kLazy || fresh) ? mn : ref;
+      const float alpha = fresh ? 1.f : __builtin_amdgcn_exp2f(ref - to);
+      ref = to;
+      l *= alpha;
+#pragma unroll
+      for (int j = 0; j < DQ; ++j) o[j] *= alpha;
+    }
+    bf16x8_t p[4];
+    float sum = 0.f;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][8 * u + 2 * i], a.scale, -ref));
+          const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][8 * u + 2 * i + 1], a.scale, -ref));
+          sum += e0 + e1;
+          const bf16x2_t v = __builtin_convertvector(f32x2_t{e0, e1}, bf16x2_t);
+          p[2 * t + u][2 * i] = v[0];
+          p[2 * t + u][2 * i + 1] = v[1];
+        }
+    l += sum;
+    const float vs = ve == 255u ? 1.f : e8m0_f32(ve);
+    // A code that is not a number reaches only the rows that see its token (see the kernel above).
+    uint32_t bad = 0u;
+#pragma unroll
+    for (int j = 0; j < DQ; ++j) {
+      const u32x4_t* vp = reinterpret_cast<const u32x4_t*>(kb + kBlock * D + ((2 * j + up) * 64 + hl * 16 + c16) * 16);
+      u32x4_t va = vp[0], vb = vp[32];
+      if constexpr (EDGE) {
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const uint32_t ba = ve == 255u ? ~0u : nan_bytes(va[w]), bb = ve == 255u ? ~0u : nan_bytes(vb[w]);
+          bad |= ba | bb;
+          va[w] &= ~ba;
+          vb[w] &= ~bb;
+        }
+      }
+#pragma unroll
+      for (int w = 0; w < 4; ++w)
+        o[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(to_bf16(va[w], vb[w], vs), p[w], o[j], 0, 0, 0);
+    }
+    if constexpr (EDGE) {
+      if (__ballot(bad != 0u)) {
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int tk = t0 + 16 * w + 8 * (i >> 2) + 4 * hl + (i & 3);
+            p[w][i] = (__bf16)(tk < hi && tk >= row_lo ? 1.f : 0.f);
+          }
+#pragma unroll
+        for (int j = 0; j < DQ; ++j) {
+          const u32x4_t* vp = reinterpret_cast<const u32x4_t*>(kb + kBlock * D + ((2 * j + up) * 64 + hl * 16 + c16) * 16);
+          const u32x4_t va = vp[0], vb = vp[32];
+          f32x16_t n;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) n[i] = 0.f;
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const uint32_t ba = ve == 255u ? ~0u : nan_bytes(va[w]), bb = ve == 255u ? ~0u : nan_bytes(vb[w]);
+            n = __builtin_amdgcn_mfma_f32_32x32x16_bf16(to_bf16(ba & 0x38383838u, bb & 0x38383838u, 1.f), p[w], n, 0, 0, 0);
+          }
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[j][i] = n[i] > 0.f ? NAN : o[j][i];
+        }
+      }
+    }
+  };
+
+  for (int b = 0; b < nblk; ++b) {
+    if (b + 1 < nblk)
+      stage_ready<CPW>();
+    else
+      stage_ready<0>();
+    const uint32_t sc_2 = issue(b + 2);
+    const int t0 = (b0 + b) * kBlock;
+    const uint32_t sc = sc_cur;
+    sc_cur = sc_next;
+    sc_next = sc_2;
+    if (t0 >= any_hi || t0 + kBlock <= any_lo) continue;
+    const bool good = sc != ~0u;
+    const uint32_t ke = good ? sc & 0xFFu : 127u, ve = good ? sc >> 8 : 127u;
+    const uint8_t* kb = buf + (b % STAGES) * STAGE;
+    if (t0 + kBlock > all_hi || t0 < all_lo || !good || ke == 255u || ve == 255u)
+      block(std::true_type{}, kb, t0, good, ke, ve);
+    else
+      block(std::false_type{}, kb, t0, true, ke, ve);
+  }
+  l = half_sum(l);
+  if (gridDim.y == 1) {
+    const float s_ = a.sink ? a.sink[head] * kLog2e : -INFINITY;
+    const float inv = m == -INFINITY ? l : 1.f / (l + __builtin_amdgcn_exp2f(s_ - ref));
+    if (c < wrows) {
+      uint16_t* orow = a.out + ((int64_t)(x.s0 + tok) * a.hq + head) * D;
+#pragma unroll
+      for (int j = 0; j < DQ; ++j)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          // dims 8 (2 i + hl) .. + 7 of 32: four of them are the other half's
+          uint32_t w[2][2];
+#pragma unroll
+          for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+              w[k][n] = (uint32_t)f32_bf16(o[j][4 * (2 * i + k) + 2 * n] * inv) |
+                        ((uint32_t)f32_bf16(o[j][4 * (2 * i + k) + 2 * n + 1] * inv) << 16);
+          const auto r0 = __builtin_amdgcn_permlane32_swap(w[0][0], w[1][0], false, false);
+          const auto r1 = __builtin_amdgcn_permlane32_swap(w[0][1], w[1][1], false, false);
+          *reinterpret_cast<u32x4_t*>(orow + 32 * j + 8 * (2 * i + hl)) = u32x4_t{r0[0], r1[0], r0[1], r1[1]};
+        }
+    }
+    return;
+  }
+  const int64_t base = ((int64_t)(want * a.hkv + h) * gridDim.y + blockIdx.y) * (ROWS / 16);
+  if (c < wrows) {
+    const int64_t slot = base + 2 * wave + up;
+#pragma unroll
+    for (int j = 0; j < DQ; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        *reinterpret_cast<f32x4_t*>(a.tile_o + (slot * 16 + c16) * D + 32 * j + 8 * i + 4 * hl) =
+            f32x4_t{o[j][4 * i], o[j][4 * i + 1], o[j][4 * i + 2], o[j][4 * i + 3]};
+    if (hl == 0) {
+      a.tile_ml[slot * 32 + c16] = m == -INFINITY ? m : ref;
+      a.tile_ml[slot * 32 + 16 + c16] = l;
+    }
+  }
+  if (blockIdx.y == 0 && tid == 0) {
+    int32_t* t = a.tile_info + 8 + ((int64_t)want * a.hkv + h) * 8;
+    t[0] = (x.s0 + row0 / a.group) * a.group + row0 % a.group;
+    t[1] = rows;
+    t[2] = gridDim.y;
+    t[3] = (int)base;
+    t[4] = (int)base + ROWS / 16;
+    t[5] = ROWS / 16;
+  }
+}
+
+constexpr int kTileWaves = 4, kTileRows = 32 * kTileWaves;
+
+// How a call is carried out, by its sizes alone (the lengths are on the GPU).
+struct Plan {
+  bool few, many;      // which kernels run
+  int rows_max;        // requests of up to so many rows are the few-row kernel's
+  int64_t few_tiles, many_tiles, splits;  // bounds of the tiles a head; splits: workgroups a many-row tile
+  int64_t o, ml, info, tile_o, tile_ml, tile_info, total;  // workspace
+};
+
+Plan plan_of(int64_t tokens, int64_t requests, int64_t hq, int64_t hkv, int64_t d, int64_t width_blocks,
+             int64_t max_new) {
+  Plan p{};
+  const int64_t group = hq / hkv, most = (max_new && max_new < tokens ? max_new : tokens) * group;
+  const int64_t some = requests < tokens ? requests : tokens;  // requests with rows
+  p.many = most > kRows;
+  p.few = !p.many || requests > 1;
+  p.rows_max = !p.many ? INT_MAX : p.few ? kRows : 0;
+  p.few_tiles = p.few ? (p.many ? some : tokens * group / kRows + some) : 0;
+  p.many_tiles = p.many ? tokens * group / kTileRows + some : 0;
+  p.splits = 1;
+  if (p.many) {
+    const int64_t groups = p.many_tiles * hkv;
+    p.splits = groups >= kGroups ? 1 : kGroups / groups;
+    if (p.splits > width_blocks / 8) p.splits = width_blocks / 8;
+    if (p.splits > 16) p.splits = 16;
+    if (p.splits < 1) p.splits = 1;
+  }
+  const int64_t slots = p.few ? 2 * kGroups : 0;
+  const int64_t tile_slots = p.splits > 1 ? p.many_tiles * hkv * p.splits * (kTileRows / kRows) : 0;
+  p.o = 0;
+  p.ml = p.o + slots * kRows * d * 4;
+  p.info = p.ml + slots * 2 * kRows * 4;
+  p.tile_o = p.info + (p.few ? 32 + p.few_tiles * hkv * 32 : 0);
+  p.tile_ml = p.tile_o + tile_slots * kRows * d * 4;
+  p.tile_info = p.tile_ml + tile_slots * 2 * kRows * 4;
+  p.total = p.tile_info + (p.splits > 1 ? 32 + p.many_tiles * hkv * 32 : 0);
+  return p;
+}
+
+template <int D, int NW>
+int launch(const AttnArgs& a, const Plan& p, int few_rows, hipStream_t st) {
+  if (p.few) {
+    MOSAIC_LAUNCH((paged_attn_rows_kernel<D, NW>), dim3(kGroups), dim3(64 * NW), 0, st, a);
+    MOSAIC_LAUNCH_CHECK("paged_attention");
+  }
+  if (p.many) {
+    MOSAIC_LAUNCH((paged_attn_tile_kernel<D, kTileWaves>), dim3((unsigned)(p.many_tiles * a.hkv), (unsigned)p.splits),
+                  dim3(64 * kTileWaves), 0, st, a);
+    MOSAIC_LAUNCH_CHECK("paged_attention");
+  }
+  if (p.few) {
+    MOSAIC_LAUNCH(paged_attn_join_kernel<D>, dim3((unsigned)p.few_tiles, (unsigned)a.hkv, (unsigned)few_rows), dim3(256),
+                  0, st, a, (const int32_t*)a.info);
+    MOSAIC_LAUNCH_CHECK("paged_attention");
+  }
+  if (p.splits > 1) {
+    AttnArgs t = a;
+    t.part_o = a.tile_o;
+    t.part_ml = a.tile_ml;
+    MOSAIC_LAUNCH(paged_attn_join_kernel<D>, dim3((unsigned)p.many_tiles, (unsigned)a.hkv, (unsigned)kTileRows),
+                  dim3(256), 0, st, t, (const int32_t*)a.tile_info);
+    MOSAIC_LAUNCH_CHECK("paged_attention");
+  }
+  return kOk;
 }
 
 bool valid(int64_t tokens, int64_t requests, int64_t hq, int64_t hkv, int64_t d) {
   return tokens >= 0 && tokens < (1 << 21) && requests >= 0 && requests <= (1 << 20) && hkv >= 1 && hkv <= 65535 &&
-         hq >= hkv && hq <= 65535 && hq % hkv == 0 && (d == 64 || d == 128 || d == 256);
+         hq >= hkv && hq <= 65535 && hq % hkv == 0 && tokens * (hq / hkv) < (1ll << 31) && (d == 64 || d == 128 || d == 256);
 }
 
 }  // namespace
@@ -458,9 +871,10 @@ bool valid(int64_t tokens, int64_t requests, int64_t hq, int64_t hkv, int64_t d)
 using namespace mosaic;
 
 extern "C" size_t mosaic_paged_attention_workspace_bytes(int64_t tokens, int64_t requests, int64_t q_heads,
-                                                         int64_t kv_heads, int64_t head_dim) {
-  if (!valid(tokens, requests, q_heads, kv_heads, head_dim)) return 0;
-  return (size_t)sizes(tokens, requests, q_heads, kv_heads, head_dim).total;
+                                                         int64_t kv_heads, int64_t head_dim, int64_t blocks,
+                                                         int64_t width, int64_t max_new) {
+  if (!valid(tokens, requests, q_heads, kv_heads, head_dim) || blocks < 1 || width < 1 || max_new < 0) return 0;
+  return (size_t)plan_of(tokens, requests, q_heads, kv_heads, head_dim, width * blocks, max_new).total;
 }
 
 extern "C" int mosaic_paged_attention(const uint16_t* q, int64_t q_token_stride, int64_t q_head_stride, int64_t tokens,
@@ -488,12 +902,13 @@ extern "C" int mosaic_paged_attention(const uint16_t* q, int64_t q_token_stride,
   MOSAIC_CHECK_ARG(((uintptr_t)q | (uintptr_t)out | (uintptr_t)codes | (uintptr_t)workspace) % 16 == 0 &&
                        (uintptr_t)scales % 2 == 0 && q_token_stride % 8 == 0 && q_head_stride % 8 == 0,
                    "paged_attention: q, out, codes and the workspace are read and written 16 bytes at a time");
-  const Sizes s = sizes(tokens, requests, q_heads, kv_heads, head_dim);
-  MOSAIC_CHECK_ARG(workspace_bytes >= (size_t)s.total, "paged_attention: workspace of %lld bytes, %lld needed",
-                   (long long)workspace_bytes, (long long)s.total);
-  MOSAIC_CHECK_ARG(s.tiles * kv_heads < (1ll << 31) / (width * blocks),
+  const Plan p = plan_of(tokens, requests, q_heads, kv_heads, head_dim, width * blocks, max_new);
+  MOSAIC_CHECK_ARG(workspace_bytes >= (size_t)p.total, "paged_attention: workspace of %lld bytes, %lld needed",
+                   (long long)workspace_bytes, (long long)p.total);
+  // the few-row kernel numbers its (tile, head, block) units in 32 bits
+  MOSAIC_CHECK_ARG(p.few_tiles * kv_heads < (1ll << 31) / (width * blocks) && p.many_tiles * kv_heads < (1ll << 31),
                    "paged_attention: %lld row tiles over tables of %lld blocks are too many for one call",
-                   (long long)(s.tiles * kv_heads), (long long)(width * blocks));
+                   (long long)((p.few_tiles + p.many_tiles) * kv_heads), (long long)(width * blocks));
   AttnArgs a{};
   a.q = q;
   a.codes = codes;
@@ -503,9 +918,15 @@ extern "C" int mosaic_paged_attention(const uint16_t* q, int64_t q_token_stride,
   a.seq = seq_lens;
   a.sink = sink;
   a.out = out;
-  a.part_o = (float*)workspace;
-  a.part_ml = a.part_o + s.part_o / 4;
-  a.info = (int32_t*)(a.part_ml + s.part_ml / 4);
+  char* ws = (char*)workspace;
+  a.part_o = (float*)(ws + p.o);
+  a.part_ml = (float*)(ws + p.ml);
+  a.info = (int32_t*)(ws + p.info);
+  a.tile_o = (float*)(ws + p.tile_o);
+  a.tile_ml = (float*)(ws + p.tile_ml);
+  a.tile_info = (int32_t*)(ws + p.tile_info);
+  a.rows_max = p.rows_max;
+  a.zero_rows = !p.few;
   a.q_tok = q_token_stride;
   a.q_head = q_head_stride;
   a.stride = table_stride;
@@ -518,13 +939,14 @@ extern "C" int mosaic_paged_attention(const uint16_t* q, int64_t q_token_stride,
   a.pages = (int)pages;
   a.nb = (int)blocks;
   a.window = (int)window;
-  a.tiles = (int)s.tiles;
-  a.scale = softmax_scale * kLog2e;
+  // a scale of zero is one too small to move a score (the masked ones stay at -inf)
+  a.scale = fmaxf(fabsf(softmax_scale) * kLog2e, 1e-37f);
+  a.sign = softmax_scale < 0.f ? -1.f : 1.f;
   const int64_t rows = (max_new && max_new < tokens ? max_new : tokens) * a.group;
-  const int z = (int)(rows < kRows ? rows : kRows);
+  const int few_rows = (int)(rows < kRows ? rows : kRows);
   switch (head_dim) {
-    case 64: return launch<64, 8>(a, z, (hipStream_t)stream);
-    case 128: return launch<128, 8>(a, z, (hipStream_t)stream);
-    default: return launch<256, 4>(a, z, (hipStream_t)stream);
+    case 64: return launch<64, 8>(a, p, few_rows, (hipStream_t)stream);
+    case 128: return launch<128, 8>(a, p, few_rows, (hipStream_t)stream);
+    default: return launch<256, 4>(a, p, few_rows, (hipStream_t)stream);
   }
 }

@@ -1204,7 +1204,8 @@ def paged_attention(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, 
         out = torch.empty(t, hq, d, dtype=torch.bfloat16, device=dev)
     elif out.shape != q.shape or out.dtype != torch.bfloat16 or not out.is_contiguous() or out.device != dev:
         raise ValueError(f"out must be a contiguous bf16 {list(q.shape)} on {dev}")
-    nbytes = _lib.lib().mosaic_paged_attention_workspace_bytes(t, r, hq, hkv, d)
+    nbytes = _lib.lib().mosaic_paged_attention_workspace_bytes(t, r, hq, hkv, d, nb, block_table.shape[1],
+                                                              int(max_new or 0))
     ws = _workspace(workspace, nbytes, dev)
     _call_on(dev, "mosaic_paged_attention", _ptr(q), q.stride(0), q.stride(1), t, hq, _ptr(codes), _ptr(scales), p, nb,
              hkv, d, _ptr(block_table), _row_stride(block_table), block_table.shape[1], _ptr(starts), _ptr(seq_lens),

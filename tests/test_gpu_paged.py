@@ -252,6 +252,42 @@ def test_attention_long_context(dev):
     _attention_case(dev, rng, 4, 2, 64, 256, [30001, 5, 12345], [1, 2, 1])
 
 
+@pytest.mark.parametrize("hq,hkv,d,page,held,new,window", [
+    (8, 1, 128, 64, [3000, 40, 0], [100, 1, 17], 0), (16, 2, 64, 128, [5000], [60], 0), (4, 4, 256, 64, [2000], [33], 0),
+    (6, 2, 128, 64, [1500, 1500], [40, 90], 700), (16, 1, 64, 64, [4000], [2], 0)])
+def test_attention_pieces_behind_long_contexts(dev, hq, hkv, d, page, held, new, window):
+    """Few tiles of many rows over a long axis: each is cut among workgroups and joined."""
+    _attention_case(dev, np.random.default_rng(d + len(held)), hq, hkv, d, page, held, new, window, sink=True)
+
+
+def test_attention_row_whose_piece_is_empty(dev):
+    """A window that leaves whole pieces of a cut tile without keys for some of its rows."""
+    _attention_case(dev, np.random.default_rng(30), 4, 1, 64, 64, [2500], [260], window=30)
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.3, 2.0])
+def test_attention_scales(dev, scale):
+    for new in ([1, 3], [90, 1]):
+        _attention_case(dev, np.random.default_rng(31), 4, 2, 64, 64, [100, 20], new, scale=scale)
+
+
+def test_attention_queries_of_unequal_size(dev):
+    """Rows from 2^-60 to 2^20 of the others, dims within a row over 2^16, rows of zeros: q in two e4m3 parts."""
+    from mosaic_amd import ops
+    rng = np.random.default_rng(32)
+    table, total, starts, seq = _batch(rng, [70], [60], 64)
+    c, s = _cache(rng, total, 1, 2, 64)
+    q = _bf16(rng, 60, 4, 64) * np.exp2(rng.integers(-16, 1, (60, 4, 64)))
+    q[::7] *= 2.0 ** -60
+    q[3::7] *= 2.0 ** 20
+    q[5, 1] = 0.0
+    q = C.round_bf16(q.astype(np.float32))
+    o = ops.paged_attention(torch.from_numpy(q).to(dev).to(torch.bfloat16), torch.from_numpy(c).to(dev),
+                            torch.from_numpy(s).to(dev), _i32(table, dev), _i32(starts, dev), _i32(seq, dev), 2.0 ** -6)
+    want, tol = P.attention(q.astype(np.float64), c, s, table, starts, seq, 2.0 ** -6)
+    assert np.all(np.abs(o.float().cpu().numpy() - want) <= tol)
+
+
 def test_attention_many_short_requests(dev):
     rng = np.random.default_rng(12)
     held = rng.integers(0, 200, 700)
