@@ -103,8 +103,8 @@ __device__ __forceinline__ bf16x8_t to_bf16(uint32_t w0, uint32_t w1, float scal
 
 // 0xFF in every byte of w that is a NaN code (0x7F or 0xFF)
 __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {
-  const uint32_t x = (w & 0x7F7F7F7Fu) + 0x01010101u;  // the high bit of a byte: it was 0x7F
-  return ((x & 0x80808080u) >> 7) * 0xFFu;
+  const uint32_t x = ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;  // the high bit of a byte: it was 0x7F
+  return x | (x - (x >> 7));
 }
 
 template <int D, int NW>
@@ -472,9 +472,20 @@ __device__ __forceinline__ float half_sum(float x) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
-__device__ __forceinline__ void lds_copy16(const void* g, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(__builtin_amdgcn_readfirstlane(lds)),
-               "v"(g) : "memory", "m0");
+// N runs of 1 KB, 16 bytes a lane, from g (one address for the wave) to LDS: the
+// immediate offset counts on both sides
+template <int N>
+__device__ __forceinline__ void lds_copy(const uint8_t* g, uint32_t lane16, uint32_t lds) {
+  static_assert(N <= 8, "two bases of four offsets");
+  if constexpr (N > 4) {
+    lds_copy<4>(g, lane16, lds);
+    lds_copy<N - 4>(g + 4096, lane16, lds + 4096);
+  } else {
+    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(lane16), "s"(g) : "memory", "m0");
+    if constexpr (N > 1) asm volatile("global_load_lds_dwordx4 %0, %1 offset:1024" ::"v"(lane16), "s"(g) : "memory");
+    if constexpr (N > 2) asm volatile("global_load_lds_dwordx4 %0, %1 offset:2048" ::"v"(lane16), "s"(g) : "memory");
+    if constexpr (N > 3) asm volatile("global_load_lds_dwordx4 %0, %1 offset:3072" ::"v"(lane16), "s"(g) : "memory");
+  }
 }
 // own copies but the last N are in LDS, own LDS reads are done, and so are the other waves'
 template <int N>
@@ -575,35 +586,37 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) paged_attn_tile_ker
       }
   }
 
-  // pages and scales of the 64 blocks from `meta` on, one a lane
+  // where the 64 blocks from `meta` on lie and their scales (~0: no page), one a lane
   const int32_t* trow = a.table + (int64_t)r * a.stride;
-  int meta = 0, pages_ = -1;
-  uint32_t scales_ = 0u;
-  auto load_meta = [&](int at) {
-    meta = at;
-    const int blk = b0 + at + lane;
-    pages_ = -1;
-    scales_ = 0u;
-    if (at + lane < nblk) {
-      pages_ = trow[blk / a.nb];
-      if (pages_ < 0 || pages_ >= a.pages) pages_ = -1;
-      const int64_t unit = ((int64_t)max(pages_, 0) * a.nb + blk % a.nb) * a.hkv + h;
-      scales_ = *reinterpret_cast<const uint16_t*>(a.scales + unit * 2);
+  int meta = 0;
+  uint32_t at_lo = 0u, at_hi = 0u, scales_ = ~0u;
+  auto load_meta = [&](int from) {
+    meta = from;
+    at_lo = at_hi = 0u;
+    scales_ = ~0u;
+    if (from + lane < nblk) {
+      const int blk = b0 + from + lane, page = trow[blk / a.nb];
+      const bool good = page >= 0 && page < a.pages;
+      const int64_t unit = ((int64_t)(good ? page : 0) * a.nb + blk % a.nb) * a.hkv + h;
+      const uint32_t sc = *reinterpret_cast<const uint16_t*>(a.scales + unit * 2);
+      scales_ = good ? sc : ~0u;
+      at_lo = (uint32_t)(unit * STAGE);
+      at_hi = (uint32_t)((unit * STAGE) >> 32);
     }
   };
-  const uint32_t lds0 = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)buf;
-  // block j into its stage; -> its scales, or ~0 where it has no page
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)buf + wave * CPW * 1024;
+  const uint8_t* codes = a.codes + wave * CPW * 1024;
+  const uint32_t lane16 = lane * 16;
+  uint32_t lds_in = lds0;
+  // block j into the next stage; -> its scales
   auto issue = [&](int j) -> uint32_t {
     if (j >= nblk) return 0u;
     if (j - meta >= 64) load_meta(j);
-    const int page = __builtin_amdgcn_readlane(pages_, j - meta);
-    const uint32_t sc = (uint32_t)__builtin_amdgcn_readlane((int)scales_, j - meta);
-    const int64_t unit = ((int64_t)max(page, 0) * a.nb + (b0 + j) % a.nb) * a.hkv + h;
-    const uint8_t* src = a.codes + unit * STAGE + (wave * CPW) * 1024 + lane * 16;
-    const uint32_t dst = lds0 + (uint32_t)(j % STAGES) * STAGE + (uint32_t)(wave * CPW) * 1024;
-#pragma unroll
-    for (int i = 0; i < CPW; ++i) lds_copy16(src + i * 1024, dst + i * 1024);
-    return page < 0 ? ~0u : sc;
+    const uint64_t at = (uint32_t)__builtin_amdgcn_readlane((int)at_lo, j - meta) |
+                        (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)at_hi, j - meta) << 32;
+    lds_copy<CPW>(codes + at, lane16, __builtin_amdgcn_readfirstlane(lds_in));
+    lds_in = lds_in == lds0 + (STAGES - 1) * STAGE ? lds0 : lds_in + STAGE;
+    return (uint32_t)__builtin_amdgcn_readlane((int)scales_, j - meta);
   };
   load_meta(0);
   uint32_t sc_cur = issue(0), sc_next = issue(1);
@@ -615,51 +628,84 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) paged_attn_tile_ker
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[j][i] = 0.f;
 
-  // one block; EDGE: some row does not see it whole, it has no page, or a scale is no number
-  auto block = [&](auto edge, const uint8_t* kb, int t0, bool good, uint32_t ke, uint32_t ve) __attribute__((always_inline)) {
-    constexpr bool EDGE = decltype(edge)::value;
+  // One block.  Kind 0: every row sees it whole; where a row's reference has to move,
+  // nothing is done and false is the answer.  Kind 1: references may move.  Kind 2:
+  // some row may not see it whole, it may have no page or a scale that is no number.
+  auto block = [&](auto kind, const uint8_t* kb, int t0, bool good, uint32_t ke, uint32_t ve) __attribute__((always_inline)) -> bool {
+    constexpr bool MOVE = decltype(kind)::value >= 1, EDGE = decltype(kind)::value == 2;
+    // all of the keys' reads go out at once, and the values' before the exponentials:
+    // one LDS latency each instead of one a product
+    u32x4_t kw[2][DG][2], vw[DQ][2];
+#pragma unroll
+    for (int g = 0; g < DG; ++g)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const u32x4_t* p = reinterpret_cast<const u32x4_t*>(kb + (((2 * t + up) * DG + g) * 64 + 2 * hl * 16 + c16) * 16);
+        kw[t][g][0] = p[0];
+        kw[t][g][1] = p[16];
+      }
+    __builtin_amdgcn_sched_barrier(0);
     f32x16_t s[2];
     const float ks = e8m0_f32(ke);
+    const f32x16_t zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
+    for (int g = 0; g < DG; ++g)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) s[t][i] = 0.f;
+      for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int g = 0; g < DG; ++g) {
-        const u32x4_t* p = reinterpret_cast<const u32x4_t*>(kb + (((2 * t + up) * DG + g) * 64 + 2 * hl * 16 + c16) * 16);
-        const u32x4_t k0 = p[0], k1 = p[16];
-        s[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(to_bf16(k0[0], k0[1], ks), qf[g][0], s[t], 0, 0, 0);
-        s[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(to_bf16(k0[2], k0[3], ks), qf[g][1], s[t], 0, 0, 0);
-        s[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(to_bf16(k1[0], k1[1], ks), qf[g][2], s[t], 0, 0, 0);
-        s[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(to_bf16(k1[2], k1[3], ks), qf[g][3], s[t], 0, 0, 0);
+        for (int t = 0; t < 2; ++t) {
+          const u32x4_t w = kw[t][g][i >> 1];
+          s[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(to_bf16(w[2 * (i & 1)], w[2 * (i & 1) + 1], ks), qf[g][i],
+                                                         g || i ? s[t] : zero, 0, 0, 0);
+        }
+    __builtin_amdgcn_sched_barrier(0);
+    auto load_values = [&]() __attribute__((always_inline)) {
+#pragma unroll
+      for (int j = 0; j < DQ; ++j) {
+        const u32x4_t* vp = reinterpret_cast<const u32x4_t*>(kb + kBlock * D + ((2 * j + up) * 64 + hl * 16 + c16) * 16);
+        vw[j][0] = vp[0];
+        vw[j][1] = vp[32];
       }
-    }
-    const int hi = good ? row_hi : 0;
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    if constexpr (!EDGE) load_values();
+    // of the lane's tokens, counted from t0 + 4 hl: those before see_hi, from see_lo on
+    const int see_hi = (good ? row_hi : 0) - t0 - 4 * hl, see_lo = row_lo - t0 - 4 * hl;
     if constexpr (EDGE) {
+      if (ke == 255u)
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) s[t][i] = NAN;
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const int p = t0 + 32 * t + 8 * (i >> 2) + 4 * hl + (i & 3);
-          const float v = ke == 255u ? NAN : s[t][i];
-          s[t][i] = p < hi && p >= row_lo ? v : -INFINITY;
+          const int p = 32 * t + 8 * (i >> 2) + (i & 3);
+          s[t][i] = p < see_hi && p >= see_lo ? s[t][i] : -INFINITY;
         }
     }
     float bm = fmaxf(s[0][0], s[1][0]);
 #pragma unroll
     for (int i = 1; i < 16; ++i) bm = fmaxf(fmaxf(bm, s[0][i]), s[1][i]);
     bm = half_max(bm);
+    const float top = fmaxf(m, bm);
+    const float mn = top == -INFINITY ? 0.f : top * a.scale;
     const bool fresh = m == -INFINITY && bm != -INFINITY;  // the first keys of a row set its reference
-    m = fmaxf(m, bm);
-    const float mn = m == -INFINITY ? 0.f : m * a.scale;
-    if (__ballot(mn - ref > kLazy || fresh)) {
-      const float to = (mn - ref > kLazy || fresh) ? mn : ref;
-      const float alpha = fresh ? 1.f : __builtin_amdgcn_exp2f(ref - to);
-      ref = to;
-      l *= alpha;
+    const bool move = mn - ref > kLazy || fresh;
+    if constexpr (MOVE) {
+      if (__ballot(move)) {
+        const float to = move ? mn : ref;
+        const float alpha = fresh ? 1.f : __builtin_amdgcn_exp2f(ref - to);
+        ref = to;
+        l *= alpha;
 #pragma unroll
-      for (int j = 0; j < DQ; ++j) o[j] *= alpha;
+        for (int j = 0; j < DQ; ++j) o[j] *= alpha;
+      }
+    } else {
+      if (__ballot(move)) return false;
     }
+    m = top;
     bf16x8_t p[4];
     float sum = 0.f;
 #pragma unroll
@@ -677,71 +723,92 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) paged_attn_tile_ker
         }
     l += sum;
     const float vs = ve == 255u ? 1.f : e8m0_f32(ve);
-    // A code that is not a number reaches only the rows that see its token (see the kernel above).
-    uint32_t bad = 0u;
-#pragma unroll
-    for (int j = 0; j < DQ; ++j) {
-      const u32x4_t* vp = reinterpret_cast<const u32x4_t*>(kb + kBlock * D + ((2 * j + up) * 64 + hl * 16 + c16) * 16);
-      u32x4_t va = vp[0], vb = vp[32];
-      if constexpr (EDGE) {
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const uint32_t ba = ve == 255u ? ~0u : nan_bytes(va[w]), bb = ve == 255u ? ~0u : nan_bytes(vb[w]);
-          bad |= ba | bb;
-          va[w] &= ~ba;
-          vb[w] &= ~bb;
-        }
-      }
-#pragma unroll
-      for (int w = 0; w < 4; ++w)
-        o[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(to_bf16(va[w], vb[w], vs), p[w], o[j], 0, 0, 0);
-    }
+    // A code that is not a number reaches only the rows that see its token (see the
+    // kernel above): it is taken out, and where a count of the seen ones is not zero,
+    // the result is not a number.
     if constexpr (EDGE) {
-      if (__ballot(bad != 0u)) {
+      __builtin_amdgcn_sched_barrier(0);
+      load_values();
+      uint32_t any = 0u;
+#pragma unroll
+      for (int j = 0; j < DQ; ++j)
+#pragma unroll
+        for (int w = 0; w < 8; ++w) any |= (vw[j][w >> 2][w & 3] & 0x7F7F7F7Fu) + 0x01010101u;
+      if (__ballot((any & 0x80808080u) != 0u || ve == 255u)) {
+        bf16x8_t see[4];
 #pragma unroll
         for (int w = 0; w < 4; ++w)
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            const int tk = t0 + 16 * w + 8 * (i >> 2) + 4 * hl + (i & 3);
-            p[w][i] = (__bf16)(tk < hi && tk >= row_lo ? 1.f : 0.f);
+            const int tk = 16 * w + 8 * (i >> 2) + (i & 3);
+            see[w][i] = (__bf16)(tk < see_hi && tk >= see_lo ? 1.f : 0.f);
           }
 #pragma unroll
         for (int j = 0; j < DQ; ++j) {
-          const u32x4_t* vp = reinterpret_cast<const u32x4_t*>(kb + kBlock * D + ((2 * j + up) * 64 + hl * 16 + c16) * 16);
-          const u32x4_t va = vp[0], vb = vp[32];
-          f32x16_t n;
-#pragma unroll
-          for (int i = 0; i < 16; ++i) n[i] = 0.f;
+          __builtin_amdgcn_sched_barrier(0);
+          f32x16_t n = zero;
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
-            const uint32_t ba = ve == 255u ? ~0u : nan_bytes(va[w]), bb = ve == 255u ? ~0u : nan_bytes(vb[w]);
-            n = __builtin_amdgcn_mfma_f32_32x32x16_bf16(to_bf16(ba & 0x38383838u, bb & 0x38383838u, 1.f), p[w], n, 0, 0, 0);
+            const uint32_t ba = ve == 255u ? ~0u : nan_bytes(vw[j][0][w]), bb = ve == 255u ? ~0u : nan_bytes(vw[j][1][w]);
+            n = __builtin_amdgcn_mfma_f32_32x32x16_bf16(to_bf16(ba & 0x38383838u, bb & 0x38383838u, 1.f), see[w], n, 0, 0, 0);
           }
 #pragma unroll
           for (int i = 0; i < 16; ++i) o[j][i] = n[i] > 0.f ? NAN : o[j][i];
         }
+        __builtin_amdgcn_sched_barrier(0);
       }
+      load_values();
+#pragma unroll
+      for (int j = 0; j < DQ; ++j)
+#pragma unroll
+        for (int w = 0; w < 8; ++w) vw[j][w >> 2][w & 3] &= ~(ve == 255u ? ~0u : nan_bytes(vw[j][w >> 2][w & 3]));
     }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int j = 0; j < DQ; ++j)
+#pragma unroll
+      for (int w = 0; w < 4; ++w)
+        o[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(to_bf16(vw[j][0][w], vw[j][1][w], vs), p[w], o[j], 0, 0, 0);
+    return true;
   };
 
-  for (int b = 0; b < nblk; ++b) {
+  // Whole blocks that move no reference run in a loop of their own, in which O
+  // stays where it is in registers; the others leave it for one turn.
+  const uint8_t* kb = buf;
+  uint32_t sc = 0u;
+  int b = 0, t0 = 0;
+  bool none = true;  // the first block always sets references
+  auto arrive = [&]() __attribute__((always_inline)) {  // block b is in LDS; the one after the next is under way
     if (b + 1 < nblk)
       stage_ready<CPW>();
     else
       stage_ready<0>();
-    const uint32_t sc_2 = issue(b + 2);
-    const int t0 = (b0 + b) * kBlock;
-    const uint32_t sc = sc_cur;
+    sc = sc_cur;
     sc_cur = sc_next;
-    sc_next = sc_2;
-    if (t0 >= any_hi || t0 + kBlock <= any_lo) continue;
+    sc_next = issue(b + 2);
+    t0 = (b0 + b) * kBlock;
+  };
+  auto leave = [&]() __attribute__((always_inline)) {
+    ++b;
+    kb = kb == buf + (STAGES - 1) * STAGE ? buf : kb + STAGE;
+  };
+  while (b < nblk) {
+    int kind = 0;
+    for (; b < nblk; leave()) {
+      arrive();
+      if (t0 >= any_hi || t0 + kBlock <= any_lo) continue;
+      const bool whole = t0 + kBlock <= all_hi && t0 >= all_lo && sc < 0xFF00u && (sc & 0xFFu) != 255u;
+      kind = !whole ? 2 : none ? 1 : block(std::integral_constant<int, 0>{}, kb, t0, true, sc & 0xFFu, sc >> 8) ? 0 : 1;
+      if (kind) break;
+    }
+    if (kind == 0) break;
+    none = false;
     const bool good = sc != ~0u;
-    const uint32_t ke = good ? sc & 0xFFu : 127u, ve = good ? sc >> 8 : 127u;
-    const uint8_t* kb = buf + (b % STAGES) * STAGE;
-    if (t0 + kBlock > all_hi || t0 < all_lo || !good || ke == 255u || ve == 255u)
-      block(std::true_type{}, kb, t0, good, ke, ve);
+    if (kind == 1)
+      block(std::integral_constant<int, 1>{}, kb, t0, true, sc & 0xFFu, sc >> 8);
     else
-      block(std::false_type{}, kb, t0, true, ke, ve);
+      block(std::integral_constant<int, 2>{}, kb, t0, good, good ? sc & 0xFFu : 127u, good ? sc >> 8 : 127u);
+    leave();
   }
   l = half_sum(l);
   if (gridDim.y == 1) {
