@@ -24,6 +24,7 @@
 
 #include <cmath>
 #include <type_traits>
+#include <utility>
 
 #include "common.h"
 #include "../../include/mosaic_amd.h"
@@ -447,7 +448,7 @@ __global__ void __launch_bounds__(256) paged_attn_join_kernel(const AttnArgs a, 
 // ---------------------------------------------------------- many rows ----
 // Requests of many rows (prompts and their pieces): a workgroup owns 32 NW rows of
 // a key head, 32 a wave, and its waves share the blocks, which are copied
-// straight into LDS, two ahead.
+// straight into LDS, three ahead.
 //
 //   scores   S^T = K Q^T in bf16 (32 x 32 x 16), codes converted with their scale as
 //            they come out of LDS.  (Codes as they are, against q in two e4m3 parts on
@@ -456,13 +457,14 @@ __global__ void __launch_bounds__(256) paged_attn_join_kernel(const AttnArgs a, 
 //   values   O^T = V^T P^T in bf16 (32 x 32 x 16), codes converted with their
 //            scale as they come out of LDS; lane (h, c) holds tokens
 //            8 i + 4 h + .. of row c, which are its operand.
-// The running reference of the exponentials follows the maximum only when it
-// has grown by more than 2^8: p is then at most 2^8, with the same relative
-// rounding, and O is seldom scaled.
+// The reference of a row's exponentials follows its maximum only when one of them
+// would be larger than 2^8: up to there the relative rounding is the same, O is
+// seldom scaled, and the exponentials need not wait for a maximum (they find out
+// themselves).
 
 typedef __attribute__((ext_vector_type(16))) float f32x16_t;
 
-constexpr float kLazy = 8.f;  // log2
+constexpr float kLazy = 256.f;
 
 __device__ __forceinline__ float half_max(float x) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -472,20 +474,26 @@ __device__ __forceinline__ float half_sum(float x) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
-// N runs of 1 KB, 16 bytes a lane, from g (one address for the wave) to LDS: the
-// immediate offset counts on both sides
-template <int N>
+// run I of 1 KB, 16 bytes a lane, of those from g (one address for the wave) to LDS;
+// the immediate offset counts on both sides
+template <int I>
 __device__ __forceinline__ void lds_copy(const uint8_t* g, uint32_t lane16, uint32_t lds) {
-  static_assert(N <= 8, "two bases of four offsets");
-  if constexpr (N > 4) {
-    lds_copy<4>(g, lane16, lds);
-    lds_copy<N - 4>(g + 4096, lane16, lds + 4096);
-  } else {
-    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(lane16), "s"(g) : "memory", "m0");
-    if constexpr (N > 1) asm volatile("global_load_lds_dwordx4 %0, %1 offset:1024" ::"v"(lane16), "s"(g) : "memory");
-    if constexpr (N > 2) asm volatile("global_load_lds_dwordx4 %0, %1 offset:2048" ::"v"(lane16), "s"(g) : "memory");
-    if constexpr (N > 3) asm volatile("global_load_lds_dwordx4 %0, %1 offset:3072" ::"v"(lane16), "s"(g) : "memory");
-  }
+  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2 offset:%3" ::"s"(lds + I / 4 * 4096), "v"(lane16),
+               "s"(g + I / 4 * 4096), "n"(I % 4 * 1024)
+               : "memory", "m0");
+}
+// f(std::integral_constant<int, 0>) .. f(<N - 1>)
+template <typename F, int... I>
+__device__ __forceinline__ void unrolled(F&& f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, typename F>
+__device__ __forceinline__ void unrolled(F&& f) {
+  unrolled(f, std::make_integer_sequence<int, N>{});
+}
+template <int N>
+__device__ __forceinline__ void lds_copies(const uint8_t* g, uint32_t lane16, uint32_t lds) {
+  unrolled<N>([&](auto i) __attribute__((always_inline)) { lds_copy<decltype(i)::value>(g, lane16, lds); });
 }
 // own copies but the last N are in LDS, own LDS reads are done, and so are the other waves'
 template <int N>
@@ -496,7 +504,7 @@ __device__ __forceinline__ void stage_ready() {
 template <int D, int NW>
 __global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) paged_attn_tile_kernel(const AttnArgs a) {
   constexpr int DG = D / 64, DQ = D / 32, ROWS = 32 * NW, STAGE = 2 * kBlock * D;
-  constexpr int STAGES = 3, CPW = STAGE / 1024 / NW;  // copies of 1 KB a wave and block
+  constexpr int STAGES = 4, CPW = STAGE / 1024 / NW;  // copies of 1 KB a wave and block
   static_assert(CPW >= 1, "every wave copies");
   __shared__ __attribute__((aligned(16))) uint8_t buf[STAGES * STAGE];
   __shared__ uint32_t sums[NW];
@@ -589,7 +597,7 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) paged_attn_tile_ker
   // where the 64 blocks from `meta` on lie and their scales (~0: no page), one a lane
   const int32_t* trow = a.table + (int64_t)r * a.stride;
   int meta = 0;
-  uint32_t at_lo = 0u, at_hi = 0u, scales_ = ~0u;
+  uint32_t at_lo = 0u, at_hi = 0u, scales_ = ~0u, sc_in = 0u;
   auto load_meta = [&](int from) {
     meta = from;
     at_lo = at_hi = 0u;
@@ -605,215 +613,261 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) paged_attn_tile_ker
     }
   };
   const uint32_t lds0 = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)buf + wave * CPW * 1024;
-  const uint8_t* codes = a.codes + wave * CPW * 1024;
   const uint32_t lane16 = lane * 16;
-  uint32_t lds_in = lds0;
-  // block j into the next stage; -> its scales
-  auto issue = [&](int j) -> uint32_t {
-    if (j >= nblk) return 0u;
+  // block j, or the last one again: every turn copies as much, so the waits are constant
+  auto locate = [&](int j) -> const uint8_t* {
+    j = min(j, nblk - 1);
     if (j - meta >= 64) load_meta(j);
     const uint64_t at = (uint32_t)__builtin_amdgcn_readlane((int)at_lo, j - meta) |
                         (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)at_hi, j - meta) << 32;
-    lds_copy<CPW>(codes + at, lane16, __builtin_amdgcn_readfirstlane(lds_in));
-    lds_in = lds_in == lds0 + (STAGES - 1) * STAGE ? lds0 : lds_in + STAGE;
-    return (uint32_t)__builtin_amdgcn_readlane((int)scales_, j - meta);
+    sc_in = (uint32_t)__builtin_amdgcn_readlane((int)scales_, j - meta);
+    return a.codes + wave * CPW * 1024 + at;
   };
-  load_meta(0);
-  uint32_t sc_cur = issue(0), sc_next = issue(1);
 
-  float m = -INFINITY, ref = 0.f, l = 0.f;  // m: of the raw scores; ref: what the exponents are taken against
+  float ref = -INFINITY, l = 0.f;  // ref: what a row's exponents are taken against
   f32x16_t o[DQ];
+  const f32x16_t zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int j = 0; j < DQ; ++j)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) o[j][i] = 0.f;
+  for (int j = 0; j < DQ; ++j) o[j] = zero;
 
-  // One block.  Kind 0: every row sees it whole; where a row's reference has to move,
-  // nothing is done and false is the answer.  Kind 1: references may move.  Kind 2:
-  // some row may not see it whole, it may have no page or a scale that is no number.
-  auto block = [&](auto kind, const uint8_t* kb, int t0, bool good, uint32_t ke, uint32_t ve) __attribute__((always_inline)) -> bool {
-    constexpr bool MOVE = decltype(kind)::value >= 1, EDGE = decltype(kind)::value == 2;
-    // all of the keys' reads go out at once, and the values' before the exponentials:
-    // one LDS latency each instead of one a product
-    u32x4_t kw[2][DG][2], vw[DQ][2];
+  u32x4_t k0[2][2], vw[DQ][2];  // k0: the keys' first 64 dims
+  f32x16_t s[2];
+  const uint8_t* src = nullptr;  // the block being copied this turn, and to where
+  uint32_t dst = lds0;
+  auto load_keys = [&](const uint8_t* kb, int g, u32x4_t (&w)[2][2]) __attribute__((always_inline)) {
 #pragma unroll
-    for (int g = 0; g < DG; ++g)
+    for (int t = 0; t < 2; ++t) {
+      const u32x4_t* p = reinterpret_cast<const u32x4_t*>(kb + (((2 * t + up) * DG + g) * 64 + 2 * hl * 16 + c16) * 16);
+      w[t][0] = p[0];
+      w[t][1] = p[16];
+    }
+  };
+  auto load_values = [&](const uint8_t* kb) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < DQ; ++j) {
+      const u32x4_t* p = reinterpret_cast<const u32x4_t*>(kb + kBlock * D + ((2 * j + up) * 64 + hl * 16 + c16) * 16);
+      vw[j][0] = p[0];
+      vw[j][1] = p[32];
+    }
+  };
+  // Scores of a block whose keys' first 64 dims are in k0; the others' reads go out
+  // 64 dims ahead.  COPY: this turn's copies between the products.
+  auto scores = [&](auto copy, const uint8_t* kb, float ks) __attribute__((always_inline)) {
+    constexpr bool COPY = decltype(copy)::value;
+    u32x4_t kw[2][2][2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) kw[0][t][i] = k0[t][i];
+    auto step = [&](auto n) __attribute__((always_inline)) {
+      constexpr int N = decltype(n)::value, g = N / 4, i = N % 4;
+      if constexpr (i == 0 && g + 1 < DG) {
+        load_keys(kb, g + 1, kw[(g + 1) % 2]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        const u32x4_t* p = reinterpret_cast<const u32x4_t*>(kb + (((2 * t + up) * DG + g) * 64 + 2 * hl * 16 + c16) * 16);
-        kw[t][g][0] = p[0];
-        kw[t][g][1] = p[16];
+        const u32x4_t w = kw[g % 2][t][i >> 1];
+        s[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(to_bf16(w[2 * (i & 1)], w[2 * (i & 1) + 1], ks), qf[g][i],
+                                                       N ? s[t] : zero, 0, 0, 0);
       }
-    __builtin_amdgcn_sched_barrier(0);
-    f32x16_t s[2];
-    const float ks = e8m0_f32(ke);
-    const f32x16_t zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int g = 0; g < DG; ++g)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const u32x4_t w = kw[t][g][i >> 1];
-          s[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(to_bf16(w[2 * (i & 1)], w[2 * (i & 1) + 1], ks), qf[g][i],
-                                                         g || i ? s[t] : zero, 0, 0, 0);
-        }
-    __builtin_amdgcn_sched_barrier(0);
-    auto load_values = [&]() __attribute__((always_inline)) {
-#pragma unroll
-      for (int j = 0; j < DQ; ++j) {
-        const u32x4_t* vp = reinterpret_cast<const u32x4_t*>(kb + kBlock * D + ((2 * j + up) * 64 + hl * 16 + c16) * 16);
-        vw[j][0] = vp[0];
-        vw[j][1] = vp[32];
+      if constexpr (COPY && N % 2 == 1 && N / 2 < CPW) {
+        __builtin_amdgcn_sched_barrier(0);
+        lds_copy<N / 2>(src, lane16, dst);
+        __builtin_amdgcn_sched_barrier(0);
       }
-      __builtin_amdgcn_sched_barrier(0);
     };
-    if constexpr (!EDGE) load_values();
-    // of the lane's tokens, counted from t0 + 4 hl: those before see_hi, from see_lo on
-    const int see_hi = (good ? row_hi : 0) - t0 - 4 * hl, see_lo = row_lo - t0 - 4 * hl;
-    if constexpr (EDGE) {
-      if (ke == 255u)
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) s[t][i] = NAN;
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int p = 32 * t + 8 * (i >> 2) + (i & 3);
-          s[t][i] = p < see_hi && p >= see_lo ? s[t][i] : -INFINITY;
-        }
-    }
+    unrolled<4 * DG>(step);
+  };
+  static_assert(CPW <= 2 * DG, "a copy for every second step");
+  auto largest = [&]() __attribute__((always_inline)) -> float {
     float bm = fmaxf(s[0][0], s[1][0]);
 #pragma unroll
     for (int i = 1; i < 16; ++i) bm = fmaxf(fmaxf(bm, s[0][i]), s[1][i]);
-    bm = half_max(bm);
-    const float top = fmaxf(m, bm);
-    const float mn = top == -INFINITY ? 0.f : top * a.scale;
-    const bool fresh = m == -INFINITY && bm != -INFINITY;  // the first keys of a row set its reference
-    const bool move = mn - ref > kLazy || fresh;
-    if constexpr (MOVE) {
-      if (__ballot(move)) {
-        const float to = move ? mn : ref;
-        const float alpha = fresh ? 1.f : __builtin_amdgcn_exp2f(ref - to);
-        ref = to;
-        l *= alpha;
+    return half_max(bm);
+  };
+  // The reference of every row moves to its maximum with these scores.  A row
+  // without one (-inf) makes its next exponential infinite, which calls for this.
+  auto move = [&]() __attribute__((always_inline)) {
+    const float top = largest() * a.scale;
+    const bool go = top > ref;
+    const float alpha = go && ref != -INFINITY ? __builtin_amdgcn_exp2f(ref - top) : 1.f;
+    ref = go ? top : ref;
+    l *= alpha;
 #pragma unroll
-        for (int j = 0; j < DQ; ++j) o[j] *= alpha;
-      }
-    } else {
-      if (__ballot(move)) return false;
-    }
-    m = top;
-    bf16x8_t p[4];
-    float sum = 0.f;
+    for (int j = 0; j < DQ; ++j) o[j] *= alpha;
+  };
+  bf16x8_t p[4];
+  // -> the lane's largest; their sum is added to l by the caller
+  float sum;
+  auto exponentials = [&](auto fused, float to) __attribute__((always_inline)) -> float {
+    // one rounding, or two: with those, the maximum's exponent is 0 however large the scores are
+    auto power = [&](float x) __attribute__((always_inline)) {
+      return __builtin_amdgcn_exp2f(decltype(fused)::value ? __builtin_fmaf(x, a.scale, -to) : x * a.scale - to);
+    };
+    float big = 0.f;
+    sum = 0.f;
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][8 * u + 2 * i], a.scale, -ref));
-          const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][8 * u + 2 * i + 1], a.scale, -ref));
+          const float e0 = power(s[t][8 * u + 2 * i]);
+          const float e1 = power(s[t][8 * u + 2 * i + 1]);
           sum += e0 + e1;
+          big = fmaxf(fmaxf(big, e0), e1);
           const bf16x2_t v = __builtin_convertvector(f32x2_t{e0, e1}, bf16x2_t);
           p[2 * t + u][2 * i] = v[0];
           p[2 * t + u][2 * i + 1] = v[1];
         }
+    return big;
+  };
+  auto products = [&](float vs) __attribute__((always_inline)) {
+#pragma unroll
+    for (int w = 0; w < 4; ++w)
+#pragma unroll
+      for (int j = 0; j < DQ; ++j)
+        o[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(to_bf16(vw[j][0][w], vw[j][1][w], vs), p[w], o[j], 0, 0, 0);
+  };
+  // A block that every row sees whole, its first keys in registers.  The values' and the
+  // next block's keys' reads go out before the exponentials, so that no product
+  // waits for LDS.  False, and nothing done, where a reference has to move.
+  auto whole_block = [&](const uint8_t* kb, const uint8_t* next, uint32_t ke, uint32_t ve) __attribute__((always_inline)) -> bool {
+    scores(std::true_type{}, kb, e8m0_f32(ke));
+    __builtin_amdgcn_sched_barrier(0);
+    load_values(kb);
+    load_keys(next, 0, k0);
+    __builtin_amdgcn_sched_barrier(0);
+    if (__ballot(exponentials(std::true_type{}, ref) > kLazy)) return false;
     l += sum;
-    const float vs = ve == 255u ? 1.f : e8m0_f32(ve);
+    __builtin_amdgcn_sched_barrier(0);
+    products(e8m0_f32(ve));
+    return true;
+  };
+  // any other: one that some row does not see whole, without a page, or of a scale that is no number
+  auto edge_block = [&](const uint8_t* kb, int t0, bool good, uint32_t ke, uint32_t ve) __attribute__((always_inline)) {
+    load_keys(kb, 0, k0);
+    scores(std::false_type{}, kb, e8m0_f32(ke));
+    // of the lane's tokens, counted from t0 + 4 hl: those before see_hi, from see_lo on
+    const int see_hi = (good ? row_hi : 0) - t0 - 4 * hl, see_lo = row_lo - t0 - 4 * hl;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int at = 32 * t + 8 * (i >> 2) + (i & 3);
+        s[t][i] = at < see_hi && at >= see_lo ? (ke == 255u ? NAN : s[t][i]) : -INFINITY;
+      }
+    move();
+    exponentials(std::false_type{}, ref == -INFINITY ? 0.f : ref);
+    l += sum;
+    __builtin_amdgcn_sched_barrier(0);
+    load_values(kb);
     // A code that is not a number reaches only the rows that see its token (see the
     // kernel above): it is taken out, and where a count of the seen ones is not zero,
     // the result is not a number.
-    if constexpr (EDGE) {
-      __builtin_amdgcn_sched_barrier(0);
-      load_values();
-      uint32_t any = 0u;
+    uint32_t any = 0u;
 #pragma unroll
-      for (int j = 0; j < DQ; ++j)
+    for (int j = 0; j < DQ; ++j)
 #pragma unroll
-        for (int w = 0; w < 8; ++w) any |= (vw[j][w >> 2][w & 3] & 0x7F7F7F7Fu) + 0x01010101u;
-      if (__ballot((any & 0x80808080u) != 0u || ve == 255u)) {
-        bf16x8_t see[4];
+      for (int w = 0; w < 8; ++w) any |= (vw[j][w >> 2][w & 3] & 0x7F7F7F7Fu) + 0x01010101u;
+    if (__ballot((any & 0x80808080u) != 0u || ve == 255u)) {
+      bf16x8_t see[4];
 #pragma unroll
-        for (int w = 0; w < 4; ++w)
+      for (int w = 0; w < 4; ++w)
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int tk = 16 * w + 8 * (i >> 2) + (i & 3);
-            see[w][i] = (__bf16)(tk < see_hi && tk >= see_lo ? 1.f : 0.f);
-          }
-#pragma unroll
-        for (int j = 0; j < DQ; ++j) {
-          __builtin_amdgcn_sched_barrier(0);
-          f32x16_t n = zero;
-#pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            const uint32_t ba = ve == 255u ? ~0u : nan_bytes(vw[j][0][w]), bb = ve == 255u ? ~0u : nan_bytes(vw[j][1][w]);
-            n = __builtin_amdgcn_mfma_f32_32x32x16_bf16(to_bf16(ba & 0x38383838u, bb & 0x38383838u, 1.f), see[w], n, 0, 0, 0);
-          }
-#pragma unroll
-          for (int i = 0; i < 16; ++i) o[j][i] = n[i] > 0.f ? NAN : o[j][i];
+        for (int i = 0; i < 8; ++i) {
+          const int at = 16 * w + 8 * (i >> 2) + (i & 3);
+          see[w][i] = (__bf16)(at < see_hi && at >= see_lo ? 1.f : 0.f);
         }
+#pragma unroll
+      for (int j = 0; j < DQ; ++j) {
         __builtin_amdgcn_sched_barrier(0);
+        f32x16_t n = zero;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const uint32_t ba = ve == 255u ? ~0u : nan_bytes(vw[j][0][w]), bb = ve == 255u ? ~0u : nan_bytes(vw[j][1][w]);
+          n = __builtin_amdgcn_mfma_f32_32x32x16_bf16(to_bf16(ba & 0x38383838u, bb & 0x38383838u, 1.f), see[w], n, 0, 0, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[j][i] = n[i] > 0.f ? NAN : o[j][i];
       }
-      load_values();
+      __builtin_amdgcn_sched_barrier(0);
+      load_values(kb);
 #pragma unroll
       for (int j = 0; j < DQ; ++j)
 #pragma unroll
         for (int w = 0; w < 8; ++w) vw[j][w >> 2][w & 3] &= ~(ve == 255u ? ~0u : nan_bytes(vw[j][w >> 2][w & 3]));
     }
-    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (int j = 0; j < DQ; ++j)
-#pragma unroll
-      for (int w = 0; w < 4; ++w)
-        o[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(to_bf16(vw[j][0][w], vw[j][1][w], vs), p[w], o[j], 0, 0, 0);
-    return true;
+    products(ve == 255u ? 1.f : e8m0_f32(ve));
   };
 
-  // Whole blocks that move no reference run in a loop of their own, in which O
-  // stays where it is in registers; the others leave it for one turn.
-  const uint8_t* kb = buf;
-  uint32_t sc = 0u;
-  int b = 0, t0 = 0;
-  bool none = true;  // the first block always sets references
-  auto arrive = [&]() __attribute__((always_inline)) {  // block b is in LDS; the one after the next is under way
-    if (b + 1 < nblk)
+  if (nblk > 0) {
+    // Turn b begins when blocks b and b + 1 are in LDS (the keys of b + 1 are read
+    // in it) and everyone is done with b - 1, whose stage takes block b + 3.
+    // Whole blocks run in a loop of their own, in which O stays where it is in
+    // registers; the others leave it for one turn.
+    load_meta(0);
+    uint32_t sc = 0u, sc1, sc2;
+    src = locate(0);
+    sc1 = sc_in;
+    lds_copies<CPW>(src, lane16, lds0);
+    src = locate(1);
+    sc2 = sc_in;
+    lds_copies<CPW>(src, lane16, lds0 + STAGE);
+    src = locate(2);
+    lds_copies<CPW>(src, lane16, lds0 + 2 * STAGE);
+    dst = lds0 + 2 * STAGE;
+    stage_ready<2 * CPW>();
+    load_keys(buf, 0, k0);
+    const uint8_t *kb = buf, *next = buf + STAGE;
+    int b = 0, t0 = 0;
+    auto arrive = [&]() __attribute__((always_inline)) {
       stage_ready<CPW>();
-    else
-      stage_ready<0>();
-    sc = sc_cur;
-    sc_cur = sc_next;
-    sc_next = issue(b + 2);
-    t0 = (b0 + b) * kBlock;
-  };
-  auto leave = [&]() __attribute__((always_inline)) {
-    ++b;
-    kb = kb == buf + (STAGES - 1) * STAGE ? buf : kb + STAGE;
-  };
-  while (b < nblk) {
-    int kind = 0;
-    for (; b < nblk; leave()) {
-      arrive();
-      if (t0 >= any_hi || t0 + kBlock <= any_lo) continue;
-      const bool whole = t0 + kBlock <= all_hi && t0 >= all_lo && sc < 0xFF00u && (sc & 0xFFu) != 255u;
-      kind = !whole ? 2 : none ? 1 : block(std::integral_constant<int, 0>{}, kb, t0, true, sc & 0xFFu, sc >> 8) ? 0 : 1;
-      if (kind) break;
+      sc = sc1;
+      sc1 = sc2;
+      sc2 = sc_in;
+      src = locate(b + 3);
+      dst = dst == lds0 + (STAGES - 1) * STAGE ? lds0 : dst + STAGE;
+      t0 = (b0 + b) * kBlock;
+    };
+    auto leave = [&]() __attribute__((always_inline)) {
+      ++b;
+      kb = next;
+      next = next == buf + (STAGES - 1) * STAGE ? buf : next + STAGE;
+    };
+    bool again = false;
+    while (b < nblk) {
+      bool edge = false;
+      for (; b < nblk; leave()) {
+        if (!again) arrive();
+        edge = t0 + kBlock > all_hi || t0 < all_lo || sc >= 0xFF00u || (sc & 0xFFu) == 255u;
+        if (edge) break;
+        const bool done = whole_block(kb, next, sc & 0xFFu, sc >> 8);
+        edge = !done && again;  // scores so large that a rounding of them is more than 8: two roundings
+        again = !done && !again;
+        if (!done) break;
+      }
+      if (again) {  // move the references, then the block once more (its copies too, to the same place)
+        load_keys(kb, 0, k0);
+        scores(std::false_type{}, kb, e8m0_f32(sc & 0xFFu));
+        move();
+        load_keys(kb, 0, k0);
+      } else if (edge) {
+        lds_copies<CPW>(src, lane16, dst);
+        const bool good = sc != ~0u;
+        if (t0 < any_hi && t0 + kBlock > any_lo)
+          edge_block(kb, t0, good, good ? sc & 0xFFu : 127u, good ? sc >> 8 : 127u);
+        load_keys(next, 0, k0);
+        leave();
+      }
     }
-    if (kind == 0) break;
-    none = false;
-    const bool good = sc != ~0u;
-    if (kind == 1)
-      block(std::integral_constant<int, 1>{}, kb, t0, true, sc & 0xFFu, sc >> 8);
-    else
-      block(std::integral_constant<int, 2>{}, kb, t0, good, good ? sc & 0xFFu : 127u, good ? sc >> 8 : 127u);
-    leave();
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no copy outlives the workgroup
   }
   l = half_sum(l);
   if (gridDim.y == 1) {
     const float s_ = a.sink ? a.sink[head] * kLog2e : -INFINITY;
-    const float inv = m == -INFINITY ? l : 1.f / (l + __builtin_amdgcn_exp2f(s_ - ref));
+    const float inv = ref == -INFINITY ? l : 1.f / (l + __builtin_amdgcn_exp2f(s_ - ref));
     if (c < wrows) {
       uint16_t* orow = a.out + ((int64_t)(x.s0 + tok) * a.hq + head) * D;
 #pragma unroll
@@ -845,7 +899,7 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) paged_attn_tile_ker
         *reinterpret_cast<f32x4_t*>(a.tile_o + (slot * 16 + c16) * D + 32 * j + 8 * i + 4 * hl) =
             f32x4_t{o[j][4 * i], o[j][4 * i + 1], o[j][4 * i + 2], o[j][4 * i + 3]};
     if (hl == 0) {
-      a.tile_ml[slot * 32 + c16] = m == -INFINITY ? m : ref;
+      a.tile_ml[slot * 32 + c16] = ref;
       a.tile_ml[slot * 32 + 16 + c16] = l;
     }
   }
