@@ -997,43 +997,52 @@ def dsa_decode_indices(pos: torch.Tensor, window: int, cidx: torch.Tensor | None
 PAGED_BLOCK = 64  # tokens that share a scale
 
 
-def _index(t: torch.Tensor, name: str, shape: tuple, device) -> torch.Tensor:
-    """An int32 index array as it is (no copy: the caller's own buffers are read and updated)."""
+# The checks of these wrappers cost as much as their small kernels: devices are
+# compared by index, and what is wrong is only spelled out once something is.
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device  # not public: see _raw_stream
+
+
+def _index(t: torch.Tensor, name: str, n: int, device: int) -> int:
+    """The address of an int32 index array [n], taken as it is (no copy: the caller's own buffers are read and updated)."""
+    if isinstance(t, torch.Tensor) and t.dtype is torch.int32 and t.dim() == 1 and t.numel() == n and \
+            t.is_contiguous() and t.get_device() == device:
+        return t.data_ptr()
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor, got {type(t).__name__}")
-    if t.dtype != torch.int32:
-        raise ValueError(f"{name}: expected int32, got {t.dtype}")
-    if t.shape != shape or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous {list(shape)}, got {list(t.shape)}")
-    if t.device != device:
-        raise ValueError(f"{name} is on {t.device}, expected {device}")
-    return t
+    raise ValueError(f"{name} must be a contiguous int32 [{n}] on cuda:{device}, got {list(t.shape)} {t.dtype} on {t.device}")
 
 
-def _table(t: torch.Tensor, rows: int, device) -> torch.Tensor:
-    """A block table [R, B] int32; its rows may be the first B entries of longer ones."""
+def _table(t: torch.Tensor, rows: int, device: int) -> tuple[int, int, int]:
+    """A block table [R, B] int32, whose rows may be the first B entries of longer ones -> (address, row stride, B)."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"block_table must be a torch.Tensor, got {type(t).__name__}")
-    if t.dtype != torch.int32 or t.dim() != 2 or t.shape[0] != rows or t.shape[1] < 1 or \
-            t.stride(1) != 1 or (rows > 1 and t.stride(0) < t.shape[1]):
-        raise ValueError(f"block_table must be [{rows}, B] int32 with unit inner stride, got {list(t.shape)} {t.dtype} "
-                         f"strides {t.stride()}")
-    if t.device != device:
-        raise ValueError(f"block_table is on {t.device}, expected {device}")
-    return t
+    if t.dtype is torch.int32 and t.dim() == 2 and t.get_device() == device:
+        (r, b), (stride, inner) = t.shape, t.stride()
+        if r == rows and b >= 1 and inner == 1 and (stride >= b or rows <= 1):
+            return t.data_ptr(), max(stride, b), b
+    raise ValueError(f"block_table must be [{rows}, B] int32 with unit inner stride on cuda:{device}, got {list(t.shape)} "
+                     f"{t.dtype} strides {t.stride()} on {t.device}")
 
 
-def _row_stride(t: torch.Tensor) -> int:
-    return max(t.stride(0), t.shape[1])
+def _requests(t: torch.Tensor, name: str) -> tuple[int, int]:
+    """(device, R) of a batch by its int32 [R] on the GPU."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor, got {type(t).__name__}")
+    device = t.get_device()
+    if device < 0 or t.dim() != 1:
+        raise ValueError(f"{name} must be a GPU tensor [R] (mosaic_amd has no CPU path), got {list(t.shape)} on {t.device}")
+    return device, t.shape[0]
 
 
-def _call_on(device: torch.device, name: str, *args) -> None:
+def _call_on(device: int, name: str, *args) -> None:
     """``_lib.call`` on the current stream of `device`, whichever device is current."""
-    if device.index == torch.cuda.current_device():
+    if device != _current_device():
+        with torch.cuda.device(device):
+            _lib.call(name, *args, _stream())
+    elif _raw_stream is None:
         _lib.call(name, *args, _stream())
-        return
-    with torch.cuda.device(device):
-        _lib.call(name, *args, _stream())
+    else:
+        _lib.call(name, *args, _raw_stream(device))
 
 
 @dataclass
@@ -1054,7 +1063,7 @@ class PagedStep:
     @classmethod
     def empty(cls, requests: int, tokens: int, device) -> "PagedStep":
         buf = torch.empty(3 * requests + 2 + 2 * tokens, dtype=torch.int32, device=device)
-        return cls(*buf.split((requests + 1, requests, 1, requests, tokens, tokens)))
+        return cls(*buf.split_with_sizes((requests + 1, requests, 1, requests, tokens, tokens)))
 
 
 def paged_step(lengths: torch.Tensor, new: torch.Tensor, block_table: torch.Tensor, tokens: int, page_size: int,
@@ -1069,30 +1078,26 @@ def paged_step(lengths: torch.Tensor, new: torch.Tensor, block_table: torch.Tens
     placed: its length stays, its ``seq_lens`` is 0, its rows have no slot.  The
     inputs other than the table are left as they are (``out`` may not share
     their memory): commit a step by copying ``lengths`` and ``free_count``."""
-    if not isinstance(lengths, torch.Tensor) or not lengths.is_cuda or lengths.dim() != 1:
-        raise ValueError("lengths must be a GPU tensor [R] (mosaic_amd has no CPU path)")
-    dev, r = lengths.device, lengths.shape[0]
-    lengths, new = _index(lengths, "lengths", (r,), dev), _index(new, "new", (r,), dev)
-    block_table = _table(block_table, r, dev)
+    dev, r = _requests(lengths, "lengths")
     if (free_pages is None) != (free_count is None):
         raise ValueError("free_pages goes with free_count")
-    pages = 0
+    pages, free, count = 0, None, None
     if free_pages is not None:
-        pages = free_pages.numel()
-        free_pages, free_count = _index(free_pages, "free_pages", (pages,), dev), _index(free_count, "free_count", (1,), dev)
+        pages = free_pages.numel() if isinstance(free_pages, torch.Tensor) else 0
+        free, count = _index(free_pages, "free_pages", pages, dev), _index(free_count, "free_count", 1, dev)
     tokens = int(tokens)
+    at, add = _index(lengths, "lengths", r, dev), _index(new, "new", r, dev)
+    table, stride, width = _table(block_table, r, dev)
     if out is None:
         if tokens < 0:
             raise ValueError(f"tokens {tokens}")
-        out = PagedStep.empty(r, tokens, dev)
+        out = PagedStep.empty(r, tokens, lengths.device)
+        ptrs = (out.starts.data_ptr(), out.lengths.data_ptr(), out.seq_lens.data_ptr(), out.positions.data_ptr(),
+                out.slots.data_ptr(), out.free_count.data_ptr())
     else:
-        for name, n in (("starts", r + 1), ("lengths", r), ("free_count", 1), ("seq_lens", r), ("positions", tokens),
-                        ("slots", tokens)):
-            _index(getattr(out, name), "out." + name, (n,), dev)
-    _call_on(dev, "mosaic_paged_step", _ptr(lengths), _ptr(new), _ptr(block_table), _row_stride(block_table),
-             _ptr(free_pages), _ptr(free_count), r, block_table.shape[1], pages, tokens, int(page_size),
-             _ptr(out.starts), _ptr(out.lengths), _ptr(out.seq_lens), _ptr(out.positions), _ptr(out.slots),
-             _ptr(out.free_count))
+        ptrs = [_index(getattr(out, name), "out." + name, n, dev) for name, n in (
+            ("starts", r + 1), ("lengths", r), ("seq_lens", r), ("positions", tokens), ("slots", tokens), ("free_count", 1))]
+    _call_on(dev, "mosaic_paged_step", at, add, table, stride, free, count, r, width, pages, tokens, page_size, *ptrs)
     return out
 
 
@@ -1101,46 +1106,47 @@ def paged_trim(lengths: torch.Tensor, keep: torch.Tensor, block_table: torch.Ten
     """Shorten requests to ``keep[r]`` tokens (0 releases one; more than it holds
     changes nothing) and push the pages behind them onto ``free_pages``, in
     place: the inverse of ``paged_step``.  -> (lengths [R], free_count [1])."""
-    if not isinstance(lengths, torch.Tensor) or not lengths.is_cuda or lengths.dim() != 1:
-        raise ValueError("lengths must be a GPU tensor [R] (mosaic_amd has no CPU path)")
-    dev, r = lengths.device, lengths.shape[0]
-    lengths, keep = _index(lengths, "lengths", (r,), dev), _index(keep, "keep", (r,), dev)
-    block_table = _table(block_table, r, dev)
+    dev, r = _requests(lengths, "lengths")
     if not isinstance(free_pages, torch.Tensor):
         raise TypeError(f"free_pages must be a torch.Tensor, got {type(free_pages).__name__}")
     pages = free_pages.numel()
-    free_pages, free_count = _index(free_pages, "free_pages", (pages,), dev), _index(free_count, "free_count", (1,), dev)
-    kept, count = torch.empty(r + 1, dtype=torch.int32, device=dev).split((r, 1))
-    _call_on(dev, "mosaic_paged_trim", _ptr(lengths), _ptr(keep), _ptr(block_table), _row_stride(block_table),
-             _ptr(free_pages), _ptr(free_count), r, block_table.shape[1], pages, int(page_size), _ptr(kept),
-             _ptr(count))
+    at, to = _index(lengths, "lengths", r, dev), _index(keep, "keep", r, dev)
+    free, had = _index(free_pages, "free_pages", pages, dev), _index(free_count, "free_count", 1, dev)
+    table, stride, width = _table(block_table, r, dev)
+    kept, count = torch.empty(r + 1, dtype=torch.int32, device=lengths.device).split_with_sizes((r, 1))
+    _call_on(dev, "mosaic_paged_trim", at, to, table, stride, free, had, r, width, pages, page_size, kept.data_ptr(),
+             count.data_ptr())
     return kept, count
 
 
-def _paged_cache(codes: torch.Tensor, scales: torch.Tensor, device) -> tuple:
+def _paged_cache(codes: torch.Tensor, scales: torch.Tensor, device: int) -> tuple:
     """codes [P, NB, Hkv, 2, 64 D] and scales [P, NB, Hkv, 2], read and written in place -> (P, NB, Hkv, D)."""
-    for t, name, dtypes in ((codes, "codes", (torch.uint8, torch.float8_e4m3fn)),
-                            (scales, "scales", (torch.uint8, torch.float8_e8m0fnu))):
+    for t, name in ((codes, "codes"), (scales, "scales")):
         if not isinstance(t, torch.Tensor):
             raise TypeError(f"{name} must be a torch.Tensor, got {type(t).__name__}")
-        if t.dtype not in dtypes or not t.is_contiguous() or t.device != device:
-            raise ValueError(f"{name} must be contiguous bytes on {device}, got {t.dtype} on {t.device}")
-    if codes.dim() != 5 or codes.shape[3] != 2 or codes.shape[4] % PAGED_BLOCK or scales.shape != codes.shape[:4]:
-        raise ValueError(f"codes must be [P, NB, Hkv, 2, 64 D] and scales [P, NB, Hkv, 2], got {list(codes.shape)} and "
-                         f"{list(scales.shape)}")
-    p, nb, hkv = codes.shape[:3]
-    return p, nb, hkv, codes.shape[4] // PAGED_BLOCK
+    if codes.dim() == 5 and codes.dtype in (torch.uint8, torch.float8_e4m3fn) and codes.is_contiguous() and \
+            scales.dtype in (torch.uint8, torch.float8_e8m0fnu) and scales.is_contiguous() and \
+            codes.get_device() == device and scales.get_device() == device:
+        p, nb, hkv, two, size = codes.shape
+        if two == 2 and size % PAGED_BLOCK == 0 and scales.shape == (p, nb, hkv, 2):
+            return p, nb, hkv, size // PAGED_BLOCK
+    raise ValueError(f"codes must be contiguous e4m3 bytes [P, NB, Hkv, 2, 64 D] and scales e8m0 bytes [P, NB, Hkv, 2] on "
+                     f"cuda:{device}, got {list(codes.shape)} {codes.dtype} on {codes.device} and {list(scales.shape)} "
+                     f"{scales.dtype} on {scales.device}")
 
 
-def _paged_rows(t: torch.Tensor, name: str) -> torch.Tensor:
-    """bf16 [T, H, D] read through its strides, or a copy where 16 bytes cannot be read at a time."""
-    if _on_device(t, name).dtype != torch.bfloat16:
-        raise ValueError(f"{name}: expected bfloat16, got {t.dtype}")
-    if t.dim() != 3:
-        raise ValueError(f"{name} must be [T, H, D], got {list(t.shape)}")
-    if t.stride(2) != 1 or t.stride(0) % 8 or t.stride(1) % 8 or t.data_ptr() % 16:
+def _paged_rows(t: torch.Tensor, name: str) -> tuple:
+    """bf16 [T, H, D] read through its strides, or a copy where 16 bytes cannot be read at a time
+    -> (tensor, address, token and head stride)."""
+    if not isinstance(t, torch.Tensor) or t.dtype is not torch.bfloat16 or t.dim() != 3 or not t.is_cuda:
+        _on_device(t, name)
+        raise ValueError(f"{name} must be bfloat16 [T, H, D], got {t.dtype} {list(t.shape)}")
+    tok, head, inner = t.stride()
+    at = t.data_ptr()
+    if inner != 1 or tok % 8 or head % 8 or at % 16:
         t = t.clone(memory_format=torch.contiguous_format)
-    return t
+        (tok, head, inner), at = t.stride(), t.data_ptr()
+    return t, at, tok, head
 
 
 def paged_kv_write(k: torch.Tensor, v: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
@@ -1151,22 +1157,19 @@ def paged_kv_write(k: torch.Tensor, v: torch.Tensor, codes: torch.Tensor, scales
     2^e with the largest magnitude at most 448 2^e.  ``starts`` and ``seq_lens`` as in
     ``PagedStep``.  A block that held tokens before keeps its scale or moves to a
     larger one; the rest of a block that begins here is zeroed."""
-    k, v = _paged_rows(k, "k"), _paged_rows(v, "v")
-    dev = k.device
-    if v.device != dev or v.shape != k.shape:
-        raise ValueError(f"k {list(k.shape)} on {dev} and v {list(v.shape)} on {v.device} do not agree")
+    (k, k_at, k_tok, k_head), (v, v_at, v_tok, v_head) = _paged_rows(k, "k"), _paged_rows(v, "v")
+    dev = k.get_device()
+    if v.get_device() != dev or v.shape != k.shape:
+        raise ValueError(f"k {list(k.shape)} on {k.device} and v {list(v.shape)} on {v.device} do not agree")
     p, nb, hkv, d = _paged_cache(codes, scales, dev)
-    t = k.shape[0]
-    if tuple(k.shape[1:]) != (hkv, d):
+    t, heads, dim = k.shape
+    if heads != hkv or dim != d:
         raise ValueError(f"k {list(k.shape)} does not match a cache of {hkv} heads of {d}")
-    if not isinstance(seq_lens, torch.Tensor) or seq_lens.dim() != 1:
-        raise ValueError("seq_lens must be a tensor [R]")
-    r = seq_lens.shape[0]
-    starts, seq_lens = _index(starts, "starts", (r + 1,), dev), _index(seq_lens, "seq_lens", (r,), dev)
-    block_table = _table(block_table, r, dev)
-    _call_on(dev, "mosaic_paged_kv_write", _ptr(k), _ptr(v), k.stride(0), k.stride(1), v.stride(0), v.stride(1), t,
-             _ptr(codes), _ptr(scales), p, nb, hkv, d, _ptr(block_table), _row_stride(block_table),
-             block_table.shape[1], _ptr(starts), _ptr(seq_lens), r)
+    r = _requests(seq_lens, "seq_lens")[1]
+    first, seq = _index(starts, "starts", r + 1, dev), _index(seq_lens, "seq_lens", r, dev)
+    table, stride, width = _table(block_table, r, dev)
+    _call_on(dev, "mosaic_paged_kv_write", k_at, v_at, k_tok, k_head, v_tok, v_head, t, codes.data_ptr(),
+             scales.data_ptr(), p, nb, hkv, d, table, stride, width, first, seq, r)
 
 
 def paged_attention(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, block_table: torch.Tensor,
@@ -1183,31 +1186,30 @@ def paged_attention(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, 
     the most rows of any request where the caller knows it (it only sizes the
     launches).  A ``workspace`` serves one call at a time: calls on other
     streams, and graphs that may replay at once, need one each."""
-    q = _paged_rows(q, "q")
-    dev = q.device
+    q, q_at, q_tok, q_head = _paged_rows(q, "q")
+    dev = q.get_device()
     p, nb, hkv, d = _paged_cache(codes, scales, dev)
     t, hq, dq = q.shape
-    if dq != d or hq % hkv or hq == 0:
+    if dq != d or hkv == 0 or hq % hkv or hq == 0:
         raise ValueError(f"q {list(q.shape)} does not match a cache of {hkv} heads of {d}")
-    if not isinstance(seq_lens, torch.Tensor) or seq_lens.dim() != 1:
-        raise ValueError("seq_lens must be a tensor [R]")
-    r = seq_lens.shape[0]
-    starts, seq_lens = _index(starts, "starts", (r + 1,), dev), _index(seq_lens, "seq_lens", (r,), dev)
-    block_table = _table(block_table, r, dev)
+    r = _requests(seq_lens, "seq_lens")[1]
+    first, seq = _index(starts, "starts", r + 1, dev), _index(seq_lens, "seq_lens", r, dev)
+    table, stride, width = _table(block_table, r, dev)
     if sink is not None:
         sink = _f32(sink, "sink")
-        if tuple(sink.shape) != (hq,) or sink.device != dev:
-            raise ValueError(f"sink must be [{hq}] on {dev}, got {list(sink.shape)} on {sink.device}")
-    if max_new is not None and max_new < 1:
+        if tuple(sink.shape) != (hq,) or sink.get_device() != dev:
+            raise ValueError(f"sink must be [{hq}] on {q.device}, got {list(sink.shape)} on {sink.device}")
+    if max_new is None:
+        max_new = 0
+    elif max_new < 1:
         raise ValueError(f"max_new {max_new}")
     if out is None:
-        out = torch.empty(t, hq, d, dtype=torch.bfloat16, device=dev)
-    elif out.shape != q.shape or out.dtype != torch.bfloat16 or not out.is_contiguous() or out.device != dev:
-        raise ValueError(f"out must be a contiguous bf16 {list(q.shape)} on {dev}")
-    nbytes = _lib.lib().mosaic_paged_attention_workspace_bytes(t, r, hq, hkv, d, nb, block_table.shape[1],
-                                                              int(max_new or 0))
-    ws = _workspace(workspace, nbytes, dev)
-    _call_on(dev, "mosaic_paged_attention", _ptr(q), q.stride(0), q.stride(1), t, hq, _ptr(codes), _ptr(scales), p, nb,
-             hkv, d, _ptr(block_table), _row_stride(block_table), block_table.shape[1], _ptr(starts), _ptr(seq_lens),
-             r, _ptr(sink), int(window), int(max_new or 0), float(softmax_scale), _ptr(out), _ptr(ws), ws.numel())
+        out = torch.empty((t, hq, d), dtype=torch.bfloat16, device=q.device)
+    elif out.shape != q.shape or out.dtype is not torch.bfloat16 or not out.is_contiguous() or out.get_device() != dev:
+        raise ValueError(f"out must be a contiguous bf16 {list(q.shape)} on {q.device}")
+    nbytes = _lib.lib().mosaic_paged_attention_workspace_bytes(t, r, hq, hkv, d, nb, width, max_new)
+    ws = _workspace(workspace, nbytes, q.device)
+    _call_on(dev, "mosaic_paged_attention", q_at, q_tok, q_head, t, hq, codes.data_ptr(), scales.data_ptr(), p, nb, hkv,
+             d, table, stride, width, first, seq, r, None if sink is None else sink.data_ptr(), window, max_new,
+             softmax_scale, out.data_ptr(), ws.data_ptr(), ws.numel())
     return out
