@@ -35,6 +35,7 @@ namespace {
 constexpr int kBlock = 64;
 constexpr int kRows = 16;           // rows of a tile
 constexpr int kGroups = 512;        // workgroups of a launch (two a CU)
+constexpr int kWhole = 16;          // blocks of a table up to which tiles are not cut
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct AttnArgs {
@@ -51,6 +52,7 @@ struct AttnArgs {
   int32_t* tile_info;
   int64_t q_tok, q_head, stride;
   int r, tokens, hq, hkv, group, width, pages, nb, window;
+  bool whole;      // few-row tiles are not cut (no join)
   int rows_max;    // requests of more rows are the many-row kernel's
   bool zero_rows;  // the many-row kernel clears what lies behind the last request
   float scale;     // |softmax scale| log2(e)
@@ -108,92 +110,123 @@ __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {
   return x | (x - (x >> 7));
 }
 
+// The units of all requests are numbered through, `units(request)` of each, and so
+// are their row tiles, `tiles(request)`.  Finds the request that holds unit
+// pick(total), with its first unit and tile; none where pick gives total or more.
+// Every workgroup does this by itself: one round trip to L2 for up to 64 NW requests.
+struct Place {
+  Request x;
+  int r, tile0;
+  uint32_t unit0, unit, total, tiles;
+};
+template <int NW, typename Units, typename Tiles, typename Pick>
+__device__ __forceinline__ Place place(const AttnArgs& a, Units units, Tiles tiles, Pick pick) {
+  __shared__ uint32_t sums[NW][2];
+  __shared__ int found[10];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  Place p{};
+  uint32_t n = 0, t = 0, at = 0, t_at = 0;
+  auto count = [&](int base) {  // this thread's request, and what lies before it
+    p.x = request_of(a, base + tid);
+    n = units(p.x);
+    t = tiles(p.x);
+    const uint32_t incl = wave_incl_scan_u32(n), tinc = wave_incl_scan_u32(t);
+    if (lane == 63) {
+      sums[wave][0] = incl;
+      sums[wave][1] = tinc;
+    }
+    __syncthreads();
+    at = p.total + incl - n;
+    t_at = p.tiles + tinc - t;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      at += w < wave ? sums[w][0] : 0u;
+      t_at += w < wave ? sums[w][1] : 0u;
+      p.total += sums[w][0];
+      p.tiles += sums[w][1];
+    }
+    __syncthreads();
+  };
+  for (int base = 0; base < a.r; base += 64 * NW) count(base);
+  const uint32_t total = __builtin_amdgcn_readfirstlane(p.total), all = __builtin_amdgcn_readfirstlane(p.tiles);
+  p.unit = pick(total);
+  if (p.unit >= total) return Place{Request{}, 0, 0, 0u, p.unit, total, all};  // nothing of a lane's own in the answer
+  auto note = [&](int base) {
+    if (p.unit >= at && p.unit - at < n) {
+      const int v[10] = {p.x.s0, p.x.n, p.x.held, p.x.first, p.x.blocks, p.x.rows, base + tid, (int)t_at, (int)at, 0};
+#pragma unroll
+      for (int i = 0; i < 9; ++i) found[i] = v[i];
+    }
+    __syncthreads();
+  };
+  if (a.r <= 64 * NW) {
+    note(0);
+  } else {
+    p.total = p.tiles = 0;
+    for (int base = 0; base < a.r && (uint32_t)__builtin_amdgcn_readfirstlane(p.total) <= p.unit; base += 64 * NW) {
+      count(base);
+      note(base);
+    }
+  }
+  auto get = [&](int i) { return __builtin_amdgcn_readfirstlane(found[i]); };
+  p.x = Request{get(0), get(1), get(2), get(3), get(4), get(5)};
+  p.r = get(6);
+  p.tile0 = get(7);
+  p.unit0 = (uint32_t)get(8);
+  p.total = total;
+  p.tiles = all;
+  return p;
+}
+
+// rows behind the last request are zero
+template <int D>
+__device__ __forceinline__ void clear_rest(const AttnArgs& a, int64_t thread, int64_t threads) {
+  const int64_t from = a.r ? min(max(a.starts[a.r], 0), a.tokens) : 0, per = (int64_t)a.hq * D;
+  for (int64_t i = from * per + 8 * thread; i < a.tokens * per; i += 8 * threads)
+    *reinterpret_cast<u32x4_t*>(a.out + i) = u32x4_t{0u, 0u, 0u, 0u};
+}
+
 template <int D, int NW>
 __global__ void __launch_bounds__(64 * NW) paged_attn_rows_kernel(const AttnArgs a) {
   constexpr int DG = D / 64, DT = D / 16;
   __shared__ __attribute__((aligned(16))) f32x4_t so[NW / 2][DT * 4 * 16];
   __shared__ float sm[NW][16], sl[NW][16];
-  __shared__ uint32_t sums[NW], sums_t[NW], s_unit;
-  __shared__ int s_req, s_tile;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, q = lane >> 4, c = lane & 15;
   const float scale = a.scale * a.sign;
 
-  // every workgroup counts the units of all requests; then the one that holds its run's first unit
-  uint32_t total = 0, tiles_all = 0;
-  for (int base = 0; base < a.r; base += 64 * NW) {
-    const Request x = request_of(a, base + tid);
-    const uint32_t t = (uint32_t)few_tiles(a, x), n = t * (uint32_t)a.hkv * (uint32_t)x.blocks;
-    const uint32_t incl = wave_incl_scan_u32(n), tinc = wave_incl_scan_u32(t);
-    if (lane == 63) {
-      sums[wave] = incl;
-      sums_t[wave] = tinc;
-    }
-    __syncthreads();
-    for (int w = 0; w < NW; ++w) {
-      total += sums[w];
-      tiles_all += sums_t[w];
-    }
-    __syncthreads();
-  }
-  const uint32_t share = max((total + kGroups - 1) / kGroups, (uint32_t)NW / 2);
-  const uint32_t u0 = blockIdx.x * share, u1 = min(u0 + share, total);
-  if (blockIdx.x == 0) {  // rows behind the last request are zero
-    if (tid == 0) a.info[0] = (int32_t)tiles_all;
-    const int64_t from = a.r ? min(max(a.starts[a.r], 0), a.tokens) : 0;
-    const int64_t per = (int64_t)a.hq * D;
-    for (int64_t i = from * per + 8 * tid; i < a.tokens * per; i += 8 * 64 * NW)
-      *reinterpret_cast<u32x4_t*>(a.out + i) = u32x4_t{0u, 0u, 0u, 0u};
-  }
-  if (u0 >= total) return;
-  {
-    uint32_t seen = 0;
-    uint32_t tiles = 0;
-    for (int base = 0; base < a.r; base += 64 * NW) {
-      const Request x = request_of(a, base + tid);
-      const uint32_t t = (uint32_t)few_tiles(a, x), n = t * (uint32_t)a.hkv * (uint32_t)x.blocks;
-      const uint32_t incl = wave_incl_scan_u32(n), tinc = wave_incl_scan_u32(t);
-      if (lane == 63) {
-        sums[wave] = incl;
-        sums_t[wave] = tinc;
-      }
-      __syncthreads();
-      uint32_t at = seen, t_at = tiles;
-      for (int w = 0; w < NW; ++w) {
-        if (w < wave) {
-          at += sums[w];
-          t_at += sums_t[w];
-        }
-        seen += sums[w];
-        tiles += sums_t[w];
-      }
-      at += incl - n;
-      if (u0 >= at && u0 - at < n) {
-        s_req = base + tid;
-        s_unit = at;
-        s_tile = (int)(t_at + tinc - t);
-      }
-      __syncthreads();
-      if (seen > u0) break;
-    }
-  }
-  __syncthreads();
-  int r = s_req, tile0 = s_tile;
-  uint32_t req0 = s_unit;
-  Request x = request_of(a, r);
-  uint32_t tiles = (uint32_t)few_tiles(a, x);
+  // units of a tile and head: its blocks, or the tile as a whole
+  auto per_tile = [&](const Request& x) { return a.whole ? 1u : (uint32_t)x.blocks; };
+  uint32_t share = 0;
+  const Place at = place<NW>(
+      a, [&](const Request& x) { return (uint32_t)few_tiles(a, x) * (uint32_t)a.hkv * per_tile(x); },
+      [&](const Request& x) { return (uint32_t)few_tiles(a, x); },
+      [&](uint32_t total) {
+        share = (total + kGroups - 1) / kGroups;
+        if (!a.whole) share = max(share, (uint32_t)NW / 2);
+        return min(blockIdx.x * (uint64_t)share, (uint64_t)total);
+      });
+  clear_rest<D>(a, (int64_t)blockIdx.x * 64 * NW + tid, (int64_t)kGroups * 64 * NW);
+  if (blockIdx.x == 0 && tid == 0) a.info[0] = a.whole ? 0 : (int32_t)at.tiles;  // what the join looks at
+  const uint32_t u0 = at.unit, u1 = min(u0 + share, at.total);
+  if (u0 >= at.total) return;
+  Request x = at.x, after = request_of(a, at.r + 1);
+  int r = at.r, tile0 = at.tile0;
+  uint32_t req0 = at.unit0, tiles = (uint32_t)few_tiles(a, x), per = per_tile(x);
   for (uint32_t u = u0; u < u1;) {
-    while (u - req0 >= tiles * (uint32_t)a.hkv * (uint32_t)x.blocks) {
-      req0 += tiles * (uint32_t)a.hkv * (uint32_t)x.blocks;
+    while (u - req0 >= tiles * (uint32_t)a.hkv * per) {
+      req0 += tiles * (uint32_t)a.hkv * per;
       tile0 += (int)tiles;
-      x = request_of(a, ++r);
+      x = after;
+      after = request_of(a, ++r + 1);  // read ahead: the next segment does not wait for it
       tiles = (uint32_t)few_tiles(a, x);
+      per = per_tile(x);
     }
     // unit -> (head, tile, block), blocks fastest
-    const uint32_t in = u - req0, ht = in / (uint32_t)x.blocks;
-    const int b_from = (int)(in % (uint32_t)x.blocks), b_to = (int)min((uint32_t)x.blocks, (uint32_t)b_from + (u1 - u));
+    const uint32_t in = u - req0, ht = in / per;
+    const int b_from = a.whole ? 0 : (int)(in % per), b_to = a.whole ? x.blocks : (int)min(per, (uint32_t)b_from + (u1 - u));
     const int h = (int)(ht / tiles), tile = (int)(ht % tiles);
     const uint32_t tile_u0 = u - b_from;
-    u += b_to - b_from;
+    u += a.whole ? 1 : b_to - b_from;
     const int row0 = tile * kRows, rows = min(kRows, x.rows - row0);
     const int row = row0 + min(c, rows - 1);
     const int tok = row / a.group, head = h * a.group + row % a.group;
@@ -355,7 +388,7 @@ __global__ void __launch_bounds__(64 * NW) paged_attn_rows_kernel(const AttnArgs
     const bool whole = b_from == 0 && b_to == x.blocks;
     // a piece that begins inside its tile is its run's first, one that only ends inside is its last
     const int slot = 2 * (int)blockIdx.x + (b_from == 0 ? 1 : 0);
-    if (b_from == 0 && tid == 0) {  // the join's list: this tile's rows and the runs that hold it
+    if (!a.whole && b_from == 0 && tid == 0) {  // the join's list: this tile's rows and the runs that hold it
       int32_t* t = a.info + 8 + ((int64_t)(tile0 + tile) * a.hkv + h) * 8;
       t[0] = (x.s0 + row0 / a.group) * a.group + row0 % a.group;
       t[1] = rows;
@@ -507,57 +540,22 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) paged_attn_tile_ker
   constexpr int STAGES = 4, CPW = STAGE / 1024 / NW;  // copies of 1 KB a wave and block
   static_assert(CPW >= 1, "every wave copies");
   __shared__ __attribute__((aligned(16))) uint8_t buf[STAGES * STAGE];
-  __shared__ uint32_t sums[NW];
-  __shared__ int s_req, s_tile;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int hl = lane >> 5, c = lane & 31, c16 = lane & 15, up = (lane >> 4) & 1;
 
-  if (a.zero_rows && blockIdx.x == 0 && blockIdx.y == 0) {
-    const int64_t from = a.r ? min(max(a.starts[a.r], 0), a.tokens) : 0, per = (int64_t)a.hq * D;
-    for (int64_t i = from * per + 8 * tid; i < a.tokens * per; i += 8 * 64 * NW)
-      *reinterpret_cast<u32x4_t*>(a.out + i) = u32x4_t{0u, 0u, 0u, 0u};
-  }
+  if (a.zero_rows && blockIdx.y == 0) clear_rest<D>(a, (int64_t)blockIdx.x * 64 * NW + tid, (int64_t)gridDim.x * 64 * NW);
   // the request and tile: key heads fastest (a head's workgroups meet in one XCD's
   // L2 where there are eight), the last tiles, which see most, first
   const int h = blockIdx.x % a.hkv;
-  uint32_t total = 0;
-  for (int base = 0; base < a.r; base += 64 * NW) {
-    const Request x = request_of(a, base + tid);
-    const uint32_t n = many_rows(a, x) ? (uint32_t)((x.rows + ROWS - 1) / ROWS) : 0u;
-    const uint32_t incl = wave_incl_scan_u32(n);
-    if (lane == 63) sums[wave] = incl;
-    __syncthreads();
-    for (int w = 0; w < NW; ++w) total += sums[w];
-    __syncthreads();
-  }
-  if (blockIdx.x == 0 && blockIdx.y == 0 && tid == 0 && gridDim.y > 1) a.tile_info[0] = (int32_t)total;
   const uint32_t idx = blockIdx.x / a.hkv;
-  if (idx >= total) return;
-  const uint32_t want = total - 1 - idx;
-  {
-    uint32_t seen = 0;
-    for (int base = 0; base < a.r; base += 64 * NW) {
-      const Request x = request_of(a, base + tid);
-      const uint32_t n = many_rows(a, x) ? (uint32_t)((x.rows + ROWS - 1) / ROWS) : 0u;
-      const uint32_t incl = wave_incl_scan_u32(n);
-      if (lane == 63) sums[wave] = incl;
-      __syncthreads();
-      uint32_t at = seen + incl - n;
-      for (int w = 0; w < NW; ++w) {
-        if (w < wave) at += sums[w];
-        seen += sums[w];
-      }
-      if (want >= at && want - at < n) {
-        s_req = base + tid;
-        s_tile = (int)(want - at);
-      }
-      __syncthreads();
-      if (seen > want) break;
-    }
-  }
-  __syncthreads();
-  const int r = __builtin_amdgcn_readfirstlane(s_req), tile = __builtin_amdgcn_readfirstlane(s_tile);
-  const Request x = request_of(a, r);
+  auto count = [&](const Request& x) { return many_rows(a, x) ? (uint32_t)((x.rows + ROWS - 1) / ROWS) : 0u; };
+  const Place found = place<NW>(a, count, [](const Request&) { return 0u; },
+                                [&](uint32_t total) { return idx < total ? total - 1 - idx : total; });
+  if (gridDim.y > 1 && blockIdx.x == 0 && blockIdx.y == 0 && tid == 0) a.tile_info[0] = (int32_t)found.total;
+  if (found.unit >= found.total) return;
+  const uint32_t want = found.unit;
+  const int r = found.r, tile = (int)(want - found.unit0);
+  const Request x = found.x;
   const int row0 = tile * ROWS, rows = min(ROWS, x.rows - row0);
   const int limit = a.width * a.nb * kBlock;
   // blocks that the tile sees, and this workgroup's share of them
@@ -919,6 +917,7 @@ constexpr int kTileWaves = 4, kTileRows = 32 * kTileWaves;
 // How a call is carried out, by its sizes alone (the lengths are on the GPU).
 struct Plan {
   bool few, many;      // which kernels run
+  bool whole;          // few-row tiles are not cut
   int rows_max;        // requests of up to so many rows are the few-row kernel's
   int64_t few_tiles, many_tiles, splits;  // bounds of the tiles a head; splits: workgroups a many-row tile
   int64_t o, ml, info, tile_o, tile_ml, tile_info, total;  // workspace
@@ -932,6 +931,8 @@ Plan plan_of(int64_t tokens, int64_t requests, int64_t hq, int64_t hkv, int64_t 
   p.many = most > kRows;
   p.few = !p.many || requests > 1;
   p.rows_max = !p.many ? INT_MAX : p.few ? kRows : 0;
+  // a table of few blocks: its tiles are a turn or two of a workgroup's waves, less than a join takes
+  p.whole = width_blocks <= kWhole;
   p.few_tiles = p.few ? (p.many ? some : tokens * group / kRows + some) : 0;
   p.many_tiles = p.many ? tokens * group / kTileRows + some : 0;
   p.splits = 1;
@@ -942,12 +943,12 @@ Plan plan_of(int64_t tokens, int64_t requests, int64_t hq, int64_t hkv, int64_t 
     if (p.splits > 16) p.splits = 16;
     if (p.splits < 1) p.splits = 1;
   }
-  const int64_t slots = p.few ? 2 * kGroups : 0;
+  const int64_t slots = p.few && !p.whole ? 2 * kGroups : 0;
   const int64_t tile_slots = p.splits > 1 ? p.many_tiles * hkv * p.splits * (kTileRows / kRows) : 0;
   p.o = 0;
   p.ml = p.o + slots * kRows * d * 4;
   p.info = p.ml + slots * 2 * kRows * 4;
-  p.tile_o = p.info + (p.few ? 32 + p.few_tiles * hkv * 32 : 0);
+  p.tile_o = p.info + (p.few ? 32 + (p.whole ? 0 : p.few_tiles * hkv * 32) : 0);
   p.tile_ml = p.tile_o + tile_slots * kRows * d * 4;
   p.tile_info = p.tile_ml + tile_slots * 2 * kRows * 4;
   p.total = p.tile_info + (p.splits > 1 ? 32 + p.many_tiles * hkv * 32 : 0);
@@ -965,7 +966,7 @@ int launch(const AttnArgs& a, const Plan& p, int few_rows, hipStream_t st) {
                   dim3(64 * kTileWaves), 0, st, a);
     MOSAIC_LAUNCH_CHECK("paged_attention");
   }
-  if (p.few) {
+  if (p.few && !p.whole) {
     MOSAIC_LAUNCH(paged_attn_join_kernel<D>, dim3((unsigned)p.few_tiles, (unsigned)a.hkv, (unsigned)few_rows), dim3(256),
                   0, st, a, (const int32_t*)a.info);
     MOSAIC_LAUNCH_CHECK("paged_attention");
@@ -1047,6 +1048,7 @@ extern "C" int mosaic_paged_attention(const uint16_t* q, int64_t q_token_stride,
   a.tile_ml = (float*)(ws + p.tile_ml);
   a.tile_info = (int32_t*)(ws + p.tile_info);
   a.rows_max = p.rows_max;
+  a.whole = p.whole;
   a.zero_rows = !p.few;
   a.q_tok = q_token_stride;
   a.q_head = q_head_stride;
