@@ -720,9 +720,9 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) paged_attn_tile_ker
         for (int i = 0; i < 4; ++i) {
           const float e0 = power(s[t][8 * u + 2 * i]);
           const float e1 = power(s[t][8 * u + 2 * i + 1]);
-          sum += e0 + e1;
           big = fmaxf(fmaxf(big, e0), e1);
           const bf16x2_t v = __builtin_convertvector(f32x2_t{e0, e1}, bf16x2_t);
+          sum = __builtin_amdgcn_fdot2_f32_bf16(v, bf16x2_t{(__bf16)1.f, (__bf16)1.f}, sum, false);
           p[2 * t + u][2 * i] = v[0];
           p[2 * t + u][2 * i + 1] = v[1];
         }
