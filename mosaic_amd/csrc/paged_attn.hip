@@ -485,6 +485,38 @@ __global__ void __launch_bounds__(256) paged_attn_join_kernel(const AttnArgs a, 
   }
 }
 
+// The same for tiles of many rows in few pieces: a group of D / 4 lanes a row, its
+// pieces one after the other.
+template <int D>
+__global__ void __launch_bounds__(256) paged_attn_join_rows_kernel(const AttnArgs a, const int32_t* __restrict__ info) {
+  constexpr int LANES = D / 4, SG = 256 / LANES;
+  const int tile = blockIdx.x, h = blockIdx.y, i = blockIdx.z * SG + threadIdx.x / LANES, d = threadIdx.x % LANES;
+  if (tile >= info[0]) return;
+  const int32_t* t = info + 8 + ((int64_t)tile * a.hkv + h) * 8;
+  if (i >= t[1]) return;
+  const int n = t[2], row = t[0] + i, head = h * a.group + row % a.group, c = i % 16;
+  const int64_t first = (int64_t)(t[3] + i / 16), step = t[5];  // the pieces' slots are evenly spaced here
+  float m = -INFINITY;
+#pragma unroll 4
+  for (int p = 0; p < n; ++p) m = fmaxf(m, a.part_ml[(first + step * p) * 32 + c]);
+  const float ref = m == -INFINITY ? 0.f : m;
+  f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+  float l = 0.f;
+#pragma unroll 4
+  for (int p = 0; p < n; ++p) {
+    const int64_t slot = first + step * p;
+    const float f = __builtin_amdgcn_exp2f(a.part_ml[slot * 32 + c] - ref);
+    l += f * a.part_ml[slot * 32 + 16 + c];
+    o += *reinterpret_cast<const f32x4_t*>(a.part_o + (slot * 16 + c) * D + 4 * d) * f;
+  }
+  const float s_ = a.sink ? a.sink[head] * kLog2e : -INFINITY;
+  const float inv = m == -INFINITY ? l : 1.f / (l + __builtin_amdgcn_exp2f(s_ - ref));
+  uint2 pk;
+  pk.x = (uint32_t)f32_bf16(o[0] * inv) | ((uint32_t)f32_bf16(o[1] * inv) << 16);
+  pk.y = (uint32_t)f32_bf16(o[2] * inv) | ((uint32_t)f32_bf16(o[3] * inv) << 16);
+  *reinterpret_cast<uint2*>(a.out + ((int64_t)(row / a.group) * a.hq + head) * D + 4 * d) = pk;
+}
+
 // ---------------------------------------------------------- many rows ----
 // Requests of many rows (prompts and their pieces): a workgroup owns 32 NW rows of
 // a key head, 32 a wave, and its waves share the blocks, which are copied
@@ -982,7 +1014,7 @@ int launch(const AttnArgs& a, const Plan& p, int few_rows, hipStream_t st) {
     AttnArgs t = a;
     t.part_o = a.tile_o;
     t.part_ml = a.tile_ml;
-    MOSAIC_LAUNCH(paged_attn_join_kernel<D>, dim3((unsigned)p.many_tiles, (unsigned)a.hkv, (unsigned)kTileRows),
+    MOSAIC_LAUNCH(paged_attn_join_rows_kernel<D>, dim3((unsigned)p.many_tiles, (unsigned)a.hkv, kTileRows * D / 1024),
                   dim3(256), 0, st, t, (const int32_t*)a.tile_info);
     MOSAIC_LAUNCH_CHECK("paged_attention");
   }
