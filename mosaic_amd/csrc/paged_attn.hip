@@ -432,26 +432,55 @@ __global__ void __launch_bounds__(64 * NW) paged_attn_rows_kernel(const AttnArgs
   }
 }
 
-// Adds up the pieces of a tile that was cut: one workgroup a row, its 256
-// threads as groups of D / 4 lanes (four dims each) that take the pieces in turn.
+// Adds up the pieces of a tile that was cut.  256 threads, in groups of D / 4 lanes
+// (four dims each).  Up to 16 pieces: a group a row, one piece after the other.
+// More (few rows over a long axis): the groups share a row's pieces and meet in LDS.
 template <int D>
 __global__ void __launch_bounds__(256) paged_attn_join_kernel(const AttnArgs a, const int32_t* __restrict__ info) {
   constexpr int LANES = D / 4, SG = 256 / LANES;
   __shared__ f32x4_t so[SG][LANES];
   __shared__ float red[4], ls[SG];
-  const int tile = blockIdx.x, h = blockIdx.y, tid = threadIdx.x;
+  const int tile = blockIdx.x, h = blockIdx.y, tid = threadIdx.x, g = tid / LANES, d = tid % LANES;
   if (tile >= info[0]) return;
   const int32_t* t = info + 8 + ((int64_t)tile * a.hkv + h) * 8;
   const int n = t[2];
   if (n == 1) return;
-  const int g = tid / LANES, d = tid % LANES;
+  const int step = t[5];
+  auto finish = [&](int row, float m, float l, f32x4_t o) {
+    const int head = h * a.group + row % a.group;
+    const float s_ = a.sink ? a.sink[head] * kLog2e : -INFINITY;
+    const float inv = m == -INFINITY ? l : 1.f / (l + __builtin_amdgcn_exp2f(s_ - m));
+    uint2 pk;
+    pk.x = (uint32_t)f32_bf16(o[0] * inv) | ((uint32_t)f32_bf16(o[1] * inv) << 16);
+    pk.y = (uint32_t)f32_bf16(o[2] * inv) | ((uint32_t)f32_bf16(o[3] * inv) << 16);
+    *reinterpret_cast<uint2*>(a.out + ((int64_t)(row / a.group) * a.hq + head) * D + 4 * d) = pk;
+  };
+  if (n <= 16) {
+    for (int i = blockIdx.z * SG + g; i < t[1]; i += gridDim.z * SG) {
+      const int64_t first = t[3] + i / 16, second = t[4] + i / 16;
+      const int c = i % 16;
+      float m = -INFINITY;
+#pragma unroll 4
+      for (int p = 0; p < n; ++p) m = fmaxf(m, a.part_ml[(p ? second + (int64_t)step * (p - 1) : first) * 32 + c]);
+      const float ref = m == -INFINITY ? 0.f : m;
+      f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+      float l = 0.f;
+#pragma unroll 4
+      for (int p = 0; p < n; ++p) {
+        const int64_t slot = p ? second + (int64_t)step * (p - 1) : first;
+        const float f = __builtin_amdgcn_exp2f(a.part_ml[slot * 32 + c] - ref);
+        l += f * a.part_ml[slot * 32 + 16 + c];
+        o += *reinterpret_cast<const f32x4_t*>(a.part_o + (slot * 16 + c) * D + 4 * d) * f;
+      }
+      finish(t[0] + i, m, l, o);
+    }
+    return;
+  }
   for (int i = blockIdx.z; i < t[1]; i += gridDim.z) {
-    const int row = t[0] + i, head = h * a.group + row % a.group;
-    const int64_t first = (int64_t)(t[3] + i / 16), second = (int64_t)(t[4] + i / 16), step = t[5];
+    const int64_t first = t[3] + i / 16, second = t[4] + i / 16;
     const int c = i % 16;
-    auto slot = [&](int p) { return p == 0 ? first : second + step * (p - 1); };
     float m = -INFINITY;
-    for (int p = tid; p < n; p += 256) m = fmaxf(m, a.part_ml[slot(p) * 32 + c]);
+    for (int p = tid; p < n; p += 256) m = fmaxf(m, a.part_ml[(p ? second + (int64_t)step * (p - 1) : first) * 32 + c]);
     m = wave_max_f32(m);
     if ((tid & 63) == 0) red[tid >> 6] = m;
     __syncthreads();
@@ -461,9 +490,10 @@ __global__ void __launch_bounds__(256) paged_attn_join_kernel(const AttnArgs a, 
     float l = 0.f;
 #pragma unroll 8
     for (int p = g; p < n; p += SG) {
-      const float f = __builtin_amdgcn_exp2f(a.part_ml[slot(p) * 32 + c] - ref);
-      l += f * a.part_ml[slot(p) * 32 + 16 + c];
-      o += *reinterpret_cast<const f32x4_t*>(a.part_o + (slot(p) * 16 + c) * D + 4 * d) * f;
+      const int64_t slot = p ? second + (int64_t)step * (p - 1) : first;
+      const float f = __builtin_amdgcn_exp2f(a.part_ml[slot * 32 + c] - ref);
+      l += f * a.part_ml[slot * 32 + 16 + c];
+      o += *reinterpret_cast<const f32x4_t*>(a.part_o + (slot * 16 + c) * D + 4 * d) * f;
     }
     so[g][d] = o;
     if (d == 0) ls[g] = l;
@@ -474,47 +504,10 @@ __global__ void __launch_bounds__(256) paged_attn_join_kernel(const AttnArgs a, 
         o += so[p][d];
         l += ls[p];
       }
-      const float s_ = a.sink ? a.sink[head] * kLog2e : -INFINITY;
-      const float inv = m == -INFINITY ? l : 1.f / (l + __builtin_amdgcn_exp2f(s_ - ref));
-      uint2 pk;
-      pk.x = (uint32_t)f32_bf16(o[0] * inv) | ((uint32_t)f32_bf16(o[1] * inv) << 16);
-      pk.y = (uint32_t)f32_bf16(o[2] * inv) | ((uint32_t)f32_bf16(o[3] * inv) << 16);
-      *reinterpret_cast<uint2*>(a.out + ((int64_t)(row / a.group) * a.hq + head) * D + 4 * d) = pk;
+      finish(t[0] + i, m, l, o);
     }
     __syncthreads();  // so, ls and red are used again
   }
-}
-
-// The same for tiles of many rows in few pieces: a group of D / 4 lanes a row, its
-// pieces one after the other.
-template <int D>
-__global__ void __launch_bounds__(256) paged_attn_join_rows_kernel(const AttnArgs a, const int32_t* __restrict__ info) {
-  constexpr int LANES = D / 4, SG = 256 / LANES;
-  const int tile = blockIdx.x, h = blockIdx.y, i = blockIdx.z * SG + threadIdx.x / LANES, d = threadIdx.x % LANES;
-  if (tile >= info[0]) return;
-  const int32_t* t = info + 8 + ((int64_t)tile * a.hkv + h) * 8;
-  if (i >= t[1]) return;
-  const int n = t[2], row = t[0] + i, head = h * a.group + row % a.group, c = i % 16;
-  const int64_t first = (int64_t)(t[3] + i / 16), step = t[5];  // the pieces' slots are evenly spaced here
-  float m = -INFINITY;
-#pragma unroll 4
-  for (int p = 0; p < n; ++p) m = fmaxf(m, a.part_ml[(first + step * p) * 32 + c]);
-  const float ref = m == -INFINITY ? 0.f : m;
-  f32x4_t o = {0.f, 0.f, 0.f, 0.f};
-  float l = 0.f;
-#pragma unroll 4
-  for (int p = 0; p < n; ++p) {
-    const int64_t slot = first + step * p;
-    const float f = __builtin_amdgcn_exp2f(a.part_ml[slot * 32 + c] - ref);
-    l += f * a.part_ml[slot * 32 + 16 + c];
-    o += *reinterpret_cast<const f32x4_t*>(a.part_o + (slot * 16 + c) * D + 4 * d) * f;
-  }
-  const float s_ = a.sink ? a.sink[head] * kLog2e : -INFINITY;
-  const float inv = m == -INFINITY ? l : 1.f / (l + __builtin_amdgcn_exp2f(s_ - ref));
-  uint2 pk;
-  pk.x = (uint32_t)f32_bf16(o[0] * inv) | ((uint32_t)f32_bf16(o[1] * inv) << 16);
-  pk.y = (uint32_t)f32_bf16(o[2] * inv) | ((uint32_t)f32_bf16(o[3] * inv) << 16);
-  *reinterpret_cast<uint2*>(a.out + ((int64_t)(row / a.group) * a.hq + head) * D + 4 * d) = pk;
 }
 
 // ---------------------------------------------------------- many rows ----
@@ -604,14 +597,16 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) paged_attn_tile_ker
   const int b0 = __builtin_amdgcn_readfirstlane(first + (int)((int64_t)all_blocks * blockIdx.y / gridDim.y));
   const int nblk = __builtin_amdgcn_readfirstlane(first + (int)((int64_t)all_blocks * (blockIdx.y + 1) / gridDim.y)) - b0;
 
-  // the wave's rows, and between which tokens all and any of them see
-  const int wrow0 = row0 + 32 * wave, wrows = min(32, rows - 32 * wave);  // wrows <= 0: a wave without rows
-  const int row = wrow0 + min(c, max(wrows, 1) - 1);
-  const int safe = min(row, x.rows - 1);
-  const int tok = safe / a.group, head = h * a.group + safe % a.group, pos = x.held + tok;
+  // Every NW-th row is a wave's: the waves meet the blocks that some row does not
+  // see together, instead of one after the other at every barrier.
+  const bool has_rows = wave < rows;
+  const int in_tile = min(NW * c + wave, rows - 1), row = row0 + in_tile;
+  const bool own_row = NW * c + wave < rows;
+  const int tok = row / a.group, head = h * a.group + row % a.group, pos = x.held + tok;
   const int row_hi = min(max(pos + 1, 0), limit), row_lo = a.window ? max(pos + 1 - a.window, 0) : 0;
-  const int tok_a = wrow0 / a.group, tok_b = (wrow0 + max(wrows, 1) - 1) / a.group;
-  const int any_hi = wrows > 0 ? max(x.held + tok_b + 1, 0) : 0, all_hi = max(x.held + tok_a + 1, 0);
+  // over the tile's rows: the tokens that any and that all of them see
+  const int tok_a = row0 / a.group, tok_b = (row0 + rows - 1) / a.group;
+  const int any_hi = has_rows ? max(x.held + tok_b + 1, 0) : 0, all_hi = max(x.held + tok_a + 1, 0);
   const int any_lo = a.window ? max(x.held + tok_a + 1 - a.window, 0) : 0;
   const int all_lo = a.window ? max(x.held + tok_b + 1 - a.window, 0) : 0;
 
@@ -905,7 +900,7 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) paged_attn_tile_ker
   if (gridDim.y == 1) {
     const float s_ = a.sink ? a.sink[head] * kLog2e : -INFINITY;
     const float inv = ref == -INFINITY ? l : 1.f / (l + __builtin_amdgcn_exp2f(s_ - ref));
-    if (c < wrows) {
+    if (own_row) {
       uint16_t* orow = a.out + ((int64_t)(x.s0 + tok) * a.hq + head) * D;
 #pragma unroll
       for (int j = 0; j < DQ; ++j)
@@ -927,17 +922,17 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) paged_attn_tile_ker
     return;
   }
   const int64_t base = ((int64_t)(want * a.hkv + h) * gridDim.y + blockIdx.y) * (ROWS / 16);
-  if (c < wrows) {
-    const int64_t slot = base + 2 * wave + up;
+  if (own_row) {
+    const int64_t slot = base + in_tile / 16, at = in_tile % 16;
 #pragma unroll
     for (int j = 0; j < DQ; ++j)
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        *reinterpret_cast<f32x4_t*>(a.tile_o + (slot * 16 + c16) * D + 32 * j + 8 * i + 4 * hl) =
+        *reinterpret_cast<f32x4_t*>(a.tile_o + (slot * 16 + at) * D + 32 * j + 8 * i + 4 * hl) =
             f32x4_t{o[j][4 * i], o[j][4 * i + 1], o[j][4 * i + 2], o[j][4 * i + 3]};
     if (hl == 0) {
-      a.tile_ml[slot * 32 + c16] = ref;
-      a.tile_ml[slot * 32 + 16 + c16] = l;
+      a.tile_ml[slot * 32 + at] = ref;
+      a.tile_ml[slot * 32 + 16 + at] = l;
     }
   }
   if (blockIdx.y == 0 && tid == 0) {
@@ -952,6 +947,9 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) paged_attn_tile_ker
 }
 
 constexpr int kTileWaves = 4, kTileRows = 32 * kTileWaves;
+// Tiles of many rows are cut where there are fewer than this many, and into
+// pieces of no fewer blocks, by the width of the tables.
+constexpr int kSplitGroups = 512, kSplitBlocks = 32;
 
 // How a call is carried out, by its sizes alone (the lengths are on the GPU).
 struct Plan {
@@ -977,8 +975,8 @@ Plan plan_of(int64_t tokens, int64_t requests, int64_t hq, int64_t hkv, int64_t 
   p.splits = 1;
   if (p.many) {
     const int64_t groups = p.many_tiles * hkv;
-    p.splits = groups >= kGroups ? 1 : kGroups / groups;
-    if (p.splits > width_blocks / 8) p.splits = width_blocks / 8;
+    p.splits = (kSplitGroups + groups - 1) / groups;
+    if (p.splits > width_blocks / kSplitBlocks) p.splits = width_blocks / kSplitBlocks;
     if (p.splits > 16) p.splits = 16;
     if (p.splits < 1) p.splits = 1;
   }
@@ -1006,15 +1004,17 @@ int launch(const AttnArgs& a, const Plan& p, int few_rows, hipStream_t st) {
     MOSAIC_LAUNCH_CHECK("paged_attention");
   }
   if (p.few && !p.whole) {
-    MOSAIC_LAUNCH(paged_attn_join_kernel<D>, dim3((unsigned)p.few_tiles, (unsigned)a.hkv, (unsigned)few_rows), dim3(256),
-                  0, st, a, (const int32_t*)a.info);
+    // few tiles are cut into many pieces: a workgroup for each row of theirs
+    const int z = p.few_tiles * a.hkv <= 64 ? few_rows : (few_rows * D + 1023) / 1024;
+    MOSAIC_LAUNCH(paged_attn_join_kernel<D>, dim3((unsigned)p.few_tiles, (unsigned)a.hkv, (unsigned)z), dim3(256), 0, st,
+                  a, (const int32_t*)a.info);
     MOSAIC_LAUNCH_CHECK("paged_attention");
   }
   if (p.splits > 1) {
     AttnArgs t = a;
     t.part_o = a.tile_o;
     t.part_ml = a.tile_ml;
-    MOSAIC_LAUNCH(paged_attn_join_rows_kernel<D>, dim3((unsigned)p.many_tiles, (unsigned)a.hkv, kTileRows * D / 1024),
+    MOSAIC_LAUNCH(paged_attn_join_kernel<D>, dim3((unsigned)p.many_tiles, (unsigned)a.hkv, kTileRows * D / 1024),
                   dim3(256), 0, st, t, (const int32_t*)a.tile_info);
     MOSAIC_LAUNCH_CHECK("paged_attention");
   }
