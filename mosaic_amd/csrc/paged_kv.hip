@@ -10,6 +10,8 @@
 //   values  [D/16 dt][4 q][16 c][4 w][4 j]:   token 16 w + 4 q + j, dim 16 dt + c
 // Values are stored transposed, four consecutive tokens a word: these are the
 // tokens whose probabilities a lane of the score tile holds.
+#include <type_traits>
+
 #include "common.h"
 #include "../../include/mosaic_amd.h"
 
@@ -216,10 +218,19 @@ __device__ __forceinline__ int scale_exp(uint32_t amax_bits) {
 __device__ __forceinline__ float pow2f(int e) {  // -126 <= e <= 127
   return __uint_as_float((uint32_t)(e + 127) << 23);
 }
-// x / 2^e as an e4m3 byte: nearest even, beyond +-448 (infinities) to +-448, NaN stays NaN
-__device__ __forceinline__ uint32_t to_e4m3(float x, float inv) {
-  const uint32_t c = e4m3_hw(fminf(fmaxf(x * inv, -448.f), 448.f));
-  return x == x ? c : 0x7Fu;
+// four values as e4m3 bytes, nearest even.  ODD: infinities go to +-448 and NaN stays
+// NaN; without it |x| is at most 448.
+template <bool ODD>
+__device__ __forceinline__ uint32_t to_e4m3(float a, float b, float c, float d) {
+  if constexpr (ODD) {
+    auto fit = [](float x) { return x == x ? fminf(fmaxf(x, -448.f), 448.f) : x; };
+    a = fit(a);
+    b = fit(b);
+    c = fit(c);
+    d = fit(d);
+  }
+  const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, lo, true);
 }
 // four codes times 2^(-down), down >= 0, each rounded to the nearest even
 __device__ __forceinline__ uint32_t rescale4(uint32_t w, float f) {
@@ -241,12 +252,11 @@ __global__ void __launch_bounds__(256) paged_kv_write_kernel(const WriteArgs a) 
   constexpr int PITCH = D + 4;  // bytes a token of the staged values
   __shared__ __attribute__((aligned(16))) uint8_t stage[kBlock * PITCH];
   __shared__ uint32_t sums[4], peak[2][4];
-  __shared__ int where[3];
+  __shared__ int where[5];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, q = lane >> 4, c = lane & 15, h = blockIdx.y;
   // which request, and which of its blocks
   uint32_t seen = 0;
   if (tid == 0) where[0] = -1;
-  __syncthreads();
   for (int base = 0; base < a.r; base += 256) {
     const int r = base + tid;
     uint32_t n = 0;
@@ -262,29 +272,21 @@ __global__ void __launch_bounds__(256) paged_kv_write_kernel(const WriteArgs a) 
     if (blockIdx.x >= at && blockIdx.x - at < n) {
       where[0] = r;
       where[1] = (seq - (s1 - s0)) / kBlock + (int)(blockIdx.x - at);
+      where[2] = s0;
+      where[3] = s1 - s0;
+      where[4] = seq - (s1 - s0);
     }
     seen += total;
     if (seen > blockIdx.x) break;
   }
   __syncthreads();
-  const int r = where[0];
-  if (r < 0) return;
-  const int block = where[1];
-  const int s0 = min(max(a.starts[r], 0), a.tokens), n = min(max(a.starts[r + 1], s0), a.tokens) - s0;
-  const int held = a.seq[r] - n;
-  if (block / a.nb >= a.width) return;
+  const int r = where[0], block = where[1], s0 = where[2], n = where[3], held = where[4];
+  if (r < 0 || block / a.nb >= a.width) return;
   const int page = a.table[(int64_t)r * a.stride + block / a.nb];
-  if (page < 0 || page >= a.pages) return;
-  const int64_t unit = ((int64_t)page * a.nb + block % a.nb) * a.heads + h;
-  uint8_t* kc = a.codes + unit * (2 * kBlock * D);
-  uint8_t* vc = kc + kBlock * D;
-  uint8_t* sc = a.scales + unit * 2;
   const int lo = max(held - kBlock * block, 0), hi = min(held + n - kBlock * block, kBlock);  // the new tokens
   const int row0 = s0 + kBlock * block - held;                                                // token row of token 0
-  const bool had = lo > 0;
-  const int was[2] = {had ? (int)sc[0] - 127 : -126, had ? (int)sc[1] - 127 : -126};
+  // the new values are under way while the page is looked up
   u32x4_t x[2][G][2];
-  uint32_t big[2] = {0u, 0u};
 #pragma unroll
   for (int part = 0; part < 2; ++part) {
     const uint16_t* src = part ? a.v + (int64_t)h * a.v_head : a.k + (int64_t)h * a.k_head;
@@ -300,6 +302,20 @@ __global__ void __launch_bounds__(256) paged_kv_write_kernel(const WriteArgs a) 
       }
     }
   }
+  if (page < 0 || page >= a.pages) return;
+  const int64_t unit = ((int64_t)page * a.nb + block % a.nb) * a.heads + h;
+  uint8_t* kc = a.codes + unit * (2 * kBlock * D);
+  uint8_t* vc = kc + kBlock * D;
+  uint8_t* sc = a.scales + unit * 2;
+  const bool had = lo > 0;
+  const int was[2] = {had ? (int)sc[0] - 127 : -126, had ? (int)sc[1] - 127 : -126};
+  u32x4_t held_v[G];  // the values that the block held, for the granules that take new ones or move
+  if (had)
+#pragma unroll
+    for (int i = 0; i < G; ++i) held_v[i] = *reinterpret_cast<const u32x4_t*>(vc + ((wave + 4 * i) * 64 + lane) * 16);
+  // the largest magnitude, by its bits; infinities and NaN, where there are some, do not count
+  uint32_t big[2] = {0u, 0u};
+  bool odd = false;
 #pragma unroll
   for (int part = 0; part < 2; ++part) {
 #pragma unroll
@@ -307,11 +323,21 @@ __global__ void __launch_bounds__(256) paged_kv_write_kernel(const WriteArgs a) 
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const uint32_t w = x[part][i][j >> 2][j & 3];
-        const uint32_t a0 = (w << 16) & 0x7FFF0000u, a1 = w & 0x7FFF0000u;
-        big[part] = max(big[part], a0 < 0x7F800000u ? a0 : 0u);
-        big[part] = max(big[part], a1 < 0x7F800000u ? a1 : 0u);
+        big[part] = max(max(big[part], (w << 16) & 0x7FFF0000u), w & 0x7FFF0000u);
       }
     big[part] = wave_max_u32(big[part]);
+    if (big[part] >= 0x7F800000u) {
+      odd = true;
+      big[part] = 0u;
+#pragma unroll
+      for (int i = 0; i < G; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const uint32_t w = x[part][i][j >> 2][j & 3], a0 = (w << 16) & 0x7FFF0000u, a1 = w & 0x7FFF0000u;
+          big[part] = max(big[part], max(a0 < 0x7F800000u ? a0 : 0u, a1 < 0x7F800000u ? a1 : 0u));
+        }
+      big[part] = wave_max_u32(big[part]);
+    }
     if (lane == 0) peak[part][wave] = big[part];
   }
   __syncthreads();
@@ -320,20 +346,26 @@ __global__ void __launch_bounds__(256) paged_kv_write_kernel(const WriteArgs a) 
   for (int part = 0; part < 2; ++part)
     e[part] = max(scale_exp(max(max(peak[part][0], peak[part][1]), max(peak[part][2], peak[part][3]))), was[part]);
   uint32_t code[2][G][4];
+  auto encode = [&](auto odd_) {
 #pragma unroll
-  for (int part = 0; part < 2; ++part) {
-    // 2^-e by halves: e = 127 (a scale that was written by someone else) has no normal inverse
-    const float i0 = pow2f(-(e[part] / 2)), i1 = pow2f(-(e[part] - e[part] / 2));
+    for (int part = 0; part < 2; ++part) {
+      // 2^-e by halves: e = 128 (a NaN scale that was written by someone else) has no normal inverse
+      const float i0 = pow2f(-(e[part] / 2)), i1 = pow2f(-(e[part] - e[part] / 2));
 #pragma unroll
-    for (int i = 0; i < G; ++i)
+      for (int i = 0; i < G; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint32_t w0 = x[part][i][j >> 1][2 * (j & 1)], w1 = x[part][i][j >> 1][2 * (j & 1) + 1];
-        const float f0 = __uint_as_float(w0 << 16) * i0, f1 = __uint_as_float(w0 & 0xFFFF0000u) * i0;
-        const float f2 = __uint_as_float(w1 << 16) * i0, f3 = __uint_as_float(w1 & 0xFFFF0000u) * i0;
-        code[part][i][j] = to_e4m3(f0, i1) | to_e4m3(f1, i1) << 8 | to_e4m3(f2, i1) << 16 | to_e4m3(f3, i1) << 24;
-      }
-  }
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t w0 = x[part][i][j >> 1][2 * (j & 1)], w1 = x[part][i][j >> 1][2 * (j & 1) + 1];
+          code[part][i][j] = to_e4m3<decltype(odd_)::value>(
+              __uint_as_float(w0 << 16) * i0 * i1, __uint_as_float(w0 & 0xFFFF0000u) * i0 * i1,
+              __uint_as_float(w1 << 16) * i0 * i1, __uint_as_float(w1 & 0xFFFF0000u) * i0 * i1);
+        }
+    }
+  };
+  if (odd)
+    encode(std::true_type{});
+  else
+    encode(std::false_type{});
   const bool grow[2] = {had && e[0] > was[0], had && e[1] > was[1]};
   const float down[2] = {grow[0] ? pow2f(max(was[0] - e[0], -126)) : 1.f, grow[1] ? pow2f(max(was[1] - e[1], -126)) : 1.f};
   // keys: a granule is 16 dims of one token
@@ -377,7 +409,7 @@ __global__ void __launch_bounds__(256) paged_kv_write_kernel(const WriteArgs a) 
     if (!had) {
       *dst = u32x4_t{fresh[0], fresh[1], fresh[2], fresh[3]};
     } else if (any || grow[1]) {
-      u32x4_t o = *dst;
+      u32x4_t o = held_v[i];
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
         uint32_t old = 0u;  // bytes of tokens held before
