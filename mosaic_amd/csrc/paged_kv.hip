@@ -19,7 +19,7 @@ namespace mosaic {
 namespace {
 
 constexpr int kBlock = 64;   // tokens of a scale
-constexpr int kTile = 1024;  // requests of a scan tile, four consecutive ones a thread
+constexpr int kRows = 1024;  // token rows a workgroup of the step
 
 // Exclusive prefix of v over the workgroup's 256 threads; `sums`: four words of
 // LDS.  total: the sum over all of them.  Two barriers.
@@ -35,17 +35,16 @@ __device__ __forceinline__ uint32_t block_excl_scan(uint32_t v, uint32_t* sums, 
   return base + incl - v;
 }
 
-// The first of n ascending values that is greater than x (n if none is).
-__device__ __forceinline__ int first_above(const uint32_t* a, int n, uint32_t x) {
-  int lo = 0, hi = n;
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (a[mid] > x)
-      hi = mid;
-    else
-      lo = mid + 1;
-  }
-  return lo;
+// The first of TILE (a power of two) ascending values that is greater than x, for N
+// x's at once (the steps' LDS latencies overlap); the last if none is.
+template <int TILE, int N>
+__device__ __forceinline__ void first_above(const uint32_t* a, const uint32_t (&x)[N], int (&at)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) at[i] = 0;
+#pragma unroll
+  for (int half = TILE / 2; half; half >>= 1)
+#pragma unroll
+    for (int i = 0; i < N; ++i) at[i] += a[at[i] + half - 1] <= x[i] ? half : 0;
 }
 
 struct StepArgs {
@@ -59,49 +58,53 @@ struct StepArgs {
 // Two prefix sums over the requests (token rows, then pages), and from them every
 // output.  Latency-bound: kilobytes of reads and writes.  One launch: each
 // workgroup scans all requests by itself (the reads come from L2) and then
-// writes its own 1024 token rows and its share of the popped pages, so no
+// writes its own 1024 token rows, four a thread, and its share of the popped pages, so no
 // workgroup waits for another; the outputs may not overlap the inputs for that.
+template <int EACH>
 __global__ void __launch_bounds__(256) paged_step_kernel(const StepArgs a) {
-  __shared__ uint32_t s_end[kTile], s_take[kTile], s_len[kTile], s_before[kTile], sums[4];
+  constexpr int TILE = 256 * EACH;  // requests of a scan, EACH consecutive ones a thread
+  __shared__ uint32_t s_end[TILE], s_take[TILE], s_len[TILE], s_before[TILE], sums[4];
   const int tid = threadIdx.x;
-  const uint32_t t0 = blockIdx.x * (uint32_t)kTile, t1 = min(t0 + kTile, a.tokens);
+  const uint32_t t0 = blockIdx.x * (uint32_t)kRows, t1 = min(t0 + kRows, a.tokens);
   const uint32_t most = a.width * a.page;
   const uint32_t free = a.free_pages ? (uint32_t)min(max(*a.free_count, 0), a.pages) : 0u;
   uint32_t tok = 0, taken = 0, used = 0;
-  for (int base = 0, tile = 0; base < a.r; base += kTile, ++tile) {
-    const int r0 = base + 4 * tid;
-    uint32_t len[4], n[4];
+  for (int base = 0, tile = 0; base < a.r; base += TILE, ++tile) {
+    const int r0 = base + EACH * tid;
+    uint32_t len[EACH], n[EACH], sum_n = 0, sum_need = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < EACH; ++i) {
       const bool in = r0 + i < a.r;
       len[i] = in ? (uint32_t)max(a.lengths[r0 + i], 0) : 0u;
       // a count past the token rows is as good as one more than they are: the sums stay in 32 bits
       n[i] = in ? min((uint32_t)max(a.add[r0 + i], 0), a.tokens + 1) : 0u;
+      sum_n += n[i];
     }
-    uint32_t total, end[4], need[4], before[4];
-    uint32_t sum = tok + block_excl_scan(n[0] + n[1] + n[2] + n[3], sums, total);
+    uint32_t total, end[EACH], need[EACH], before[EACH];
+    uint32_t sum = tok + block_excl_scan(sum_n, sums, total);
     const uint32_t tok_end = min(tok + total, a.tokens + 1);
-    bool fits[4];
+    bool fits[EACH];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < EACH; ++i) {
       sum += n[i];
       end[i] = sum;
       fits[i] = sum <= a.tokens && len[i] + n[i] <= most;
       before[i] = (len[i] + a.page - 1) / a.page;
       need[i] = fits[i] ? (len[i] + n[i] + a.page - 1) / a.page - before[i] : 0u;
+      sum_need += need[i];
     }
-    uint32_t pop = taken + block_excl_scan(need[0] + need[1] + need[2] + need[3], sums, total);
+    uint32_t pop = taken + block_excl_scan(sum_need, sums, total);
     const uint32_t taken_end = taken + total;
     const bool mine = blockIdx.x == (uint32_t)tile % gridDim.x;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < EACH; ++i) {
       pop += need[i];
       const bool placed = fits[i] && (!a.free_pages || need[i] == 0 || pop <= free);
       if (placed && need[i] && a.free_pages) used = max(used, pop);
-      s_end[4 * tid + i] = end[i];
-      s_take[4 * tid + i] = pop;
-      s_len[4 * tid + i] = len[i];
-      s_before[4 * tid + i] = before[i] | (placed ? 0x80000000u : 0u);
+      s_end[EACH * tid + i] = end[i];
+      s_take[EACH * tid + i] = pop;
+      s_len[EACH * tid + i] = len[i];
+      s_before[EACH * tid + i] = before[i] | (placed ? 0x80000000u : 0u);
       if (mine && r0 + i < a.r) {
         a.starts[r0 + i + 1] = (int32_t)min(end[i], a.tokens);
         a.lengths_out[r0 + i] = (int32_t)(placed ? len[i] + n[i] : len[i]);
@@ -109,29 +112,39 @@ __global__ void __launch_bounds__(256) paged_step_kernel(const StepArgs a) {
       }
     }
     __syncthreads();
-    const int in_tile = min(kTile, a.r - base);
-    for (uint32_t t = max(t0, tok) + tid; t < min(t1, tok_end); t += 256) {
-      const int i = first_above(s_end, in_tile, t);
-      int32_t pos = -1, slot = -1;
-      if (i < in_tile && (s_before[i] >> 31)) {
-        const uint32_t old_pages = s_before[i] & 0x7FFFFFFFu, l = s_len[i];
-        const uint32_t p = l + t - (i ? s_end[i - 1] : tok);
-        const uint32_t at = p / a.page;
-        pos = (int32_t)p;
-        int32_t id;
-        if (at < old_pages || !a.free_pages)
-          id = a.table[(int64_t)(base + i) * a.stride + at];
-        else
-          id = a.free_pages[free - 1 - ((i ? s_take[i - 1] : taken) + at - old_pages)];
-        slot = (int32_t)((uint32_t)id * a.page + p % a.page);
+    if (max(t0, tok) < min(t1, tok_end)) {  // the workgroup has rows of this tile: four a thread
+      constexpr int N = kRows / 256;
+      uint32_t row[N], slot[N];
+      int at[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i) row[i] = t0 + tid + 256 * i;
+      first_above<TILE, N>(s_end, row, at);
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const uint32_t t = row[i], old_pages = s_before[at[i]] & 0x7FFFFFFFu;
+        const bool here = t >= tok && t < min(t1, tok_end), placed = here && (s_before[at[i]] >> 31);
+        const uint32_t p = s_len[at[i]] + t - (at[i] ? s_end[at[i] - 1] : tok), page = p / a.page;
+        int32_t id = 0;
+        if (placed) {
+          if (page < old_pages || !a.free_pages)
+            id = a.table[(int64_t)(base + at[i]) * a.stride + page];
+          else
+            id = a.free_pages[free - 1 - ((at[i] ? s_take[at[i] - 1] : taken) + page - old_pages)];
+        }
+        slot[i] = placed ? (uint32_t)id * a.page + p % a.page : ~0u;
+        if (here) a.positions[t] = placed ? (int32_t)p : -1;
       }
-      a.positions[t] = pos;
-      a.slots[t] = slot;
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (row[i] >= tok && row[i] < min(t1, tok_end)) a.slots[row[i]] = (int32_t)slot[i];
     }
     if (a.free_pages)
       for (uint32_t k = taken + blockIdx.x * 256 + tid; k < min(taken_end, free); k += gridDim.x * 256) {
-        const int i = first_above(s_take, in_tile, k);
-        if (i < in_tile && (s_before[i] >> 31))
+        const uint32_t ks[1] = {k};
+        int at[1];
+        first_above<TILE, 1>(s_take, ks, at);
+        const int i = at[0];
+        if (s_before[i] >> 31)
           a.table[(int64_t)(base + i) * a.stride + (s_before[i] & 0x7FFFFFFFu) + k - (i ? s_take[i - 1] : taken)] =
               a.free_pages[free - 1 - k];
       }
@@ -162,39 +175,47 @@ struct TrimArgs {
 // The inverse of popping: requests are walked from the last to the first and
 // their pages from the last to the first, so that a step taken back leaves the
 // stack as it was.  Every workgroup scans all requests, as in the step.
+template <int EACH>
 __global__ void __launch_bounds__(256) paged_trim_kernel(const TrimArgs a) {
-  __shared__ uint32_t s_take[kTile], s_last[kTile], sums[4];
+  constexpr int TILE = 256 * EACH;  // requests of a scan, EACH consecutive ones a thread
+  __shared__ uint32_t s_take[TILE], s_last[TILE], sums[4];
   const int tid = threadIdx.x;
   const uint32_t most = a.width * a.page;
   const uint32_t free = (uint32_t)min(max(*a.free_count, 0), a.pages);
   uint32_t taken = 0;
-  for (int base = 0, tile = 0; base < a.r; base += kTile, ++tile) {
-    uint32_t back[4], last[4], keep[4];
+  for (int base = 0, tile = 0; base < a.r; base += TILE, ++tile) {
+    uint32_t back[EACH], last[EACH], keep[EACH], sum_back = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = a.r - 1 - (base + 4 * tid + i);
+    for (int i = 0; i < EACH; ++i) {
+      const int r = a.r - 1 - (base + EACH * tid + i);
       const uint32_t held = r >= 0 ? min((uint32_t)max(a.lengths[r], 0), most) : 0u;
       keep[i] = r >= 0 ? min((uint32_t)max(a.keep[r], 0), held) : 0u;
       last[i] = (held + a.page - 1) / a.page;
       back[i] = last[i] - (keep[i] + a.page - 1) / a.page;
+      sum_back += back[i];
     }
     uint32_t total;
-    uint32_t sum = taken + block_excl_scan(back[0] + back[1] + back[2] + back[3], sums, total);
+    uint32_t sum = taken + block_excl_scan(sum_back, sums, total);
     const bool mine = blockIdx.x == (uint32_t)tile % gridDim.x;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < EACH; ++i) {
       sum += back[i];
-      s_take[4 * tid + i] = sum;
-      s_last[4 * tid + i] = last[i];
-      const int r = a.r - 1 - (base + 4 * tid + i);
+      s_take[EACH * tid + i] = sum;
+      s_last[EACH * tid + i] = last[i];
+      const int r = a.r - 1 - (base + EACH * tid + i);
       if (mine && r >= 0) a.lengths_out[r] = (int32_t)keep[i];
     }
     __syncthreads();
-    const int in_tile = min(kTile, a.r - base);
-    for (uint32_t k = taken + blockIdx.x * 256 + tid; k < taken + total; k += gridDim.x * 256) {
-      const int i = first_above(s_take, in_tile, k);
-      const uint32_t col = s_last[i] - 1 - (k - (i ? s_take[i - 1] : taken));
-      if (free + k < (uint32_t)a.pages) a.free_pages[free + k] = a.table[(int64_t)(a.r - 1 - (base + i)) * a.stride + col];
+    // four pages a thread and turn
+    for (uint32_t k0 = taken + blockIdx.x * 1024 + tid; k0 < taken + total; k0 += gridDim.x * 1024) {
+      const uint32_t k[4] = {k0, k0 + 256, k0 + 512, k0 + 768};
+      int i[4];
+      first_above<TILE, 4>(s_take, k, i);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (k[j] < taken + total && free + k[j] < (uint32_t)a.pages)
+          a.free_pages[free + k[j]] =
+              a.table[(int64_t)(a.r - 1 - (base + i[j])) * a.stride + s_last[i[j]] - 1 - (k[j] - (i[j] ? s_take[i[j] - 1] : taken))];
     }
     __syncthreads();
     taken += total;
@@ -462,8 +483,13 @@ extern "C" int mosaic_paged_step(const int32_t* lengths, const int32_t* add, int
   StepArgs a{lengths, add, free_pages, free_count, block_table, starts, lengths_out, seq_lens, positions, slots,
              count_out, table_stride, (int)requests, (int)(free_pages ? pages : 0), (uint32_t)width,
              (uint32_t)page_size, (uint32_t)tokens};
-  const unsigned grid = (unsigned)(tokens > kTile ? (tokens + kTile - 1) / kTile : 1);
-  MOSAIC_LAUNCH(paged_step_kernel, dim3(grid), dim3(256), 0, (hipStream_t)stream, a);
+  const unsigned grid = (unsigned)(tokens > kRows ? (tokens + kRows - 1) / kRows : 1);
+  // one request a thread is read at once (16 requests: 4.4 us, with eight 6.5), eight
+  // need one scan for 2048 of them (in two of 1024: 11.4 us, so 9.3)
+  if (requests <= 256)
+    MOSAIC_LAUNCH(paged_step_kernel<1>, dim3(grid), dim3(256), 0, (hipStream_t)stream, a);
+  else
+    MOSAIC_LAUNCH(paged_step_kernel<8>, dim3(grid), dim3(256), 0, (hipStream_t)stream, a);
   MOSAIC_RETURN_LAUNCH("paged_step");
 }
 
@@ -490,9 +516,12 @@ extern "C" int mosaic_paged_trim(const int32_t* lengths, const int32_t* keep, co
       MOSAIC_CHECK_ARG(!overlap(in[i], 4 * in_n[i], out[o], 4 * out_n[o]), "paged_trim: an output overlaps an input");
   TrimArgs a{lengths, keep, block_table, free_count, free_pages, lengths_out, count_out, table_stride,
              (int)requests, (int)pages, (uint32_t)width, (uint32_t)page_size};
-  const int64_t most = (pages < requests * width ? pages : requests * width) / kTile;
+  const int64_t most = (pages < requests * width ? pages : requests * width) / 1024;
   const unsigned grid = (unsigned)(most < 1 ? 1 : most > 128 ? 128 : most);
-  MOSAIC_LAUNCH(paged_trim_kernel, dim3(grid), dim3(256), 0, (hipStream_t)stream, a);
+  if (requests <= 256)
+    MOSAIC_LAUNCH(paged_trim_kernel<1>, dim3(grid), dim3(256), 0, (hipStream_t)stream, a);
+  else
+    MOSAIC_LAUNCH(paged_trim_kernel<8>, dim3(grid), dim3(256), 0, (hipStream_t)stream, a);
   MOSAIC_RETURN_LAUNCH("paged_trim");
 }
 

@@ -42,7 +42,9 @@ def _pool(rng, lengths, after, page, spare):
     (1, 1, 1, 64, 0, False, True), (1, 0, 1, 64, 3, False, True), (16, 500, 1, 64, 0, False, True),
     (7, 300, 200, 128, 5, False, True), (64, 1000, 3, 192, 0, True, True), (1024, 200, 2, 64, 1, False, True),
     (1025, 200, 5, 64, 0, True, True), (2500, 90, 20, 64, 77, False, True), (3, 5000, 4000, 64, 0, False, True),
-    (300, 64, 130, 64, 0, True, True), (40, 400, 60, 256, 2, False, False), (5, 70, 0, 64, 4, False, True)])
+    (300, 64, 130, 64, 0, True, True), (40, 400, 60, 256, 2, False, False), (5, 70, 0, 64, 4, False, True),
+    (256, 300, 40, 64, 9, False, True), (257, 300, 40, 64, 0, True, True), (2048, 130, 3, 64, 0, False, True),
+    (2049, 130, 3, 64, 2, True, True), (4500, 70, 2, 64, 1, False, True)])
 def test_step(dev, r, most, n, page, pad, dry, allocate):
     from mosaic_amd import ops
     rng = np.random.default_rng(r + most + n)
@@ -90,7 +92,8 @@ def test_step_without_requests(dev):
     assert s.starts.tolist() == [0] and s.positions.tolist() == [-1] * 5 and s.free_count.tolist() == [2]
 
 
-@pytest.mark.parametrize("r,most,page", [(1, 500, 64), (33, 2000, 64), (1024, 300, 128), (1030, 700, 64), (2100, 64, 64)])
+@pytest.mark.parametrize("r,most,page", [(1, 500, 64), (33, 2000, 64), (1024, 300, 128), (1030, 700, 64), (2100, 64, 64), (256, 900, 64), (257, 900, 64),
+                                         (2048, 200, 64), (4100, 100, 64)])
 def test_trim(dev, r, most, page):
     from mosaic_amd import ops
     rng = np.random.default_rng(r)
