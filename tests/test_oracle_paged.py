@@ -155,7 +155,7 @@ def _attn(**kw):
     (dict(tokens=1 << 21), "tokens"), (dict(blocks=0), "blocks"), (dict(window=-1), "window"), (dict(new=-1), "max_new"),
     (dict(scale=float("nan")), "finite"), (dict(scale=float("inf")), "finite"), (dict(qt=260), "16 bytes"),
     (dict(q=ctypes.c_void_p(4104)), "16 bytes"), (dict(out=ctypes.c_void_p(4104)), "16 bytes"),
-    (dict(scales=ctypes.c_void_p(4097)), "16 bytes"), (dict(nws=1000), "workspace"), (dict(out=None), "null"),
+    (dict(scales=ctypes.c_void_p(4097)), "16 bytes"), (dict(width=200, stride=200, nws=1000), "workspace"), (dict(nws=31), "workspace"), (dict(out=None), "null"),
     (dict(stride=1), "tables")])
 def test_attention_refusals(kw, text):
     _refused("mosaic_paged_attention", _attn(**kw), text)
