@@ -965,7 +965,7 @@ Plan plan_of(int64_t tokens, int64_t requests, int64_t hq, int64_t hkv, int64_t 
   Plan p{};
   const int64_t group = hq / hkv, most = (max_new && max_new < tokens ? max_new : tokens) * group;
   const int64_t some = requests < tokens ? requests : tokens;  // requests with rows
-  p.many = most > kRows;
+  p.many = some > 0 && most > kRows;
   p.few = !p.many || requests > 1;
   p.rows_max = !p.many ? INT_MAX : p.few ? kRows : 0;
   // a table of few blocks: its tiles are a turn or two of a workgroup's waves, less than a join takes
@@ -1049,7 +1049,7 @@ extern "C" int mosaic_paged_attention(const uint16_t* q, int64_t q_token_stride,
                    "paged_attention: %lld query heads on %lld key heads of %lld (64, 128 or 256), %lld tokens (below "
                    "2^21) of %lld requests",
                    (long long)q_heads, (long long)kv_heads, (long long)head_dim, (long long)tokens, (long long)requests);
-  MOSAIC_CHECK_ARG(pages >= 0 && pages < (1ll << 31) && blocks >= 1 && blocks <= 64,
+  MOSAIC_CHECK_ARG(pages >= 1 && pages < (1ll << 31) && blocks >= 1 && blocks <= 64,
                    "paged_attention: %lld pages of %lld blocks", (long long)pages, (long long)blocks);
   MOSAIC_CHECK_ARG(width >= 1 && width * blocks * kBlock < (1ll << 30) && table_stride >= width,
                    "paged_attention: tables of %lld pages", (long long)width);
@@ -1057,8 +1057,7 @@ extern "C" int mosaic_paged_attention(const uint16_t* q, int64_t q_token_stride,
   MOSAIC_CHECK_ARG(max_new >= 0, "paged_attention: max_new %lld", (long long)max_new);
   MOSAIC_CHECK_ARG(std::isfinite(softmax_scale), "paged_attention: the softmax scale is not finite");
   if (tokens == 0) return kOk;
-  MOSAIC_CHECK_ARG(q && out && starts && workspace && (requests == 0 || (block_table && seq_lens)) &&
-                       (pages == 0 || (codes && scales)),
+  MOSAIC_CHECK_ARG(q && out && starts && workspace && (requests == 0 || (block_table && seq_lens)) && codes && scales,
                    "paged_attention: null pointer");
   MOSAIC_CHECK_ARG(((uintptr_t)q | (uintptr_t)out | (uintptr_t)codes | (uintptr_t)workspace) % 16 == 0 &&
                        (uintptr_t)scales % 2 == 0 && q_token_stride % 8 == 0 && q_head_stride % 8 == 0,
@@ -1100,7 +1099,7 @@ extern "C" int mosaic_paged_attention(const uint16_t* q, int64_t q_token_stride,
   a.width = (int)width;
   a.pages = (int)pages;
   a.nb = (int)blocks;
-  a.window = (int)window;
+  a.window = window >= (1 << 30) ? 0 : (int)window;  // longer than any context: none
   // a scale of zero is one too small to move a score (the masked ones stay at -inf)
   a.scale = fmaxf(fabsf(softmax_scale) * kLog2e, 1e-37f);
   a.sign = softmax_scale < 0.f ? -1.f : 1.f;

@@ -355,6 +355,28 @@ def test_attention_unplaced_requests_give_zeros(dev):
     assert not o[[0, 1, 3, 4, 5]].any() and o[2].abs().max() > 0
 
 
+def test_attention_without_requests_clears_its_rows(dev):
+    from mosaic_amd import ops
+    c, s = _cache(np.random.default_rng(33), 2, 1, 1, 64)
+    for t, hq in ((1, 1), (3, 8), (300, 4)):
+        q = torch.ones(t, hq, 64, dtype=torch.bfloat16, device=dev)
+        out = torch.full_like(q, float("nan"))
+        ops.paged_attention(q, torch.from_numpy(c).to(dev), torch.from_numpy(s).to(dev),
+                            torch.zeros(0, 3, dtype=torch.int32, device=dev), _i32([0], dev), _i32([], dev), 1.0, out=out)
+        assert not out.any()
+
+
+@pytest.mark.parametrize("max_new", [1, 2, 500])
+def test_attention_holds_with_a_wrong_max_new(dev, max_new):
+    """max_new sizes the launches only: requests of more rows than it says are done all the same."""
+    _attention_case(dev, np.random.default_rng(34), 8, 2, 64, 64, [1500, 40, 0], [3, 70, 12], max_new=max_new, pad=1)
+
+
+@pytest.mark.parametrize("window", [1, 64, 2 ** 30 - 1, 2 ** 31 - 1])
+def test_attention_windows(dev, window):
+    _attention_case(dev, np.random.default_rng(35), 4, 2, 64, 64, [130, 0], [1, 90], window=window)
+
+
 def test_attention_starts_outside_the_rows(dev):
     """Starts that pass the rows are cut: no row outside is read or written."""
     from mosaic_amd import ops
