@@ -209,7 +209,7 @@ __global__ void __launch_bounds__(64 * NW) paged_attn_rows_kernel(const AttnArgs
         return min(blockIdx.x * (uint64_t)share, (uint64_t)total);
       });
   clear_rest<D>(a, (int64_t)blockIdx.x * 64 * NW + tid, (int64_t)kGroups * 64 * NW);
-  if (blockIdx.x == 0 && tid == 0) a.info[0] = a.whole ? 0 : (int32_t)at.tiles;  // what the join looks at
+  if (!a.whole && blockIdx.x == 0 && tid == 0) a.info[0] = (int32_t)at.tiles;
   const uint32_t u0 = at.unit, u1 = min(u0 + share, at.total);
   if (u0 >= at.total) return;
   Request x = at.x, after = request_of(a, at.r + 1);
@@ -985,7 +985,7 @@ Plan plan_of(int64_t tokens, int64_t requests, int64_t hq, int64_t hkv, int64_t 
   p.o = 0;
   p.ml = p.o + slots * kRows * d * 4;
   p.info = p.ml + slots * 2 * kRows * 4;
-  p.tile_o = p.info + (p.few ? 32 + (p.whole ? 0 : p.few_tiles * hkv * 32) : 0);
+  p.tile_o = p.info + (p.few && !p.whole ? 32 + p.few_tiles * hkv * 32 : 0);
   p.tile_ml = p.tile_o + tile_slots * kRows * d * 4;
   p.tile_info = p.tile_ml + tile_slots * 2 * kRows * 4;
   p.total = p.tile_info + (p.splits > 1 ? 32 + p.many_tiles * hkv * 32 : 0);
@@ -1057,13 +1057,13 @@ extern "C" int mosaic_paged_attention(const uint16_t* q, int64_t q_token_stride,
   MOSAIC_CHECK_ARG(max_new >= 0, "paged_attention: max_new %lld", (long long)max_new);
   MOSAIC_CHECK_ARG(std::isfinite(softmax_scale), "paged_attention: the softmax scale is not finite");
   if (tokens == 0) return kOk;
-  MOSAIC_CHECK_ARG(q && out && starts && workspace && (requests == 0 || (block_table && seq_lens)) && codes && scales,
+  MOSAIC_CHECK_ARG(q && out && starts && (requests == 0 || (block_table && seq_lens)) && codes && scales,
                    "paged_attention: null pointer");
   MOSAIC_CHECK_ARG(((uintptr_t)q | (uintptr_t)out | (uintptr_t)codes | (uintptr_t)workspace) % 16 == 0 &&
                        (uintptr_t)scales % 2 == 0 && q_token_stride % 8 == 0 && q_head_stride % 8 == 0,
                    "paged_attention: q, out, codes and the workspace are read and written 16 bytes at a time");
   const Plan p = plan_of(tokens, requests, q_heads, kv_heads, head_dim, width * blocks, max_new);
-  MOSAIC_CHECK_ARG(workspace_bytes >= (size_t)p.total, "paged_attention: workspace of %lld bytes, %lld needed",
+  MOSAIC_CHECK_ARG(p.total == 0 || (workspace && workspace_bytes >= (size_t)p.total), "paged_attention: workspace of %lld bytes, %lld needed",
                    (long long)workspace_bytes, (long long)p.total);
   // the few-row kernel numbers its (tile, head, block) units in 32 bits
   MOSAIC_CHECK_ARG(p.few_tiles * kv_heads < (1ll << 31) / (width * blocks) && p.many_tiles * kv_heads < (1ll << 31),

@@ -1002,11 +1002,16 @@ PAGED_BLOCK = 64  # tokens that share a scale
 _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device  # not public: see _raw_stream
 
 
+_INT32 = torch.int32
+
+
 def _index(t: torch.Tensor, name: str, n: int, device: int) -> int:
     """The address of an int32 index array [n], taken as it is (no copy: the caller's own buffers are read and updated)."""
-    if isinstance(t, torch.Tensor) and t.dtype is torch.int32 and t.dim() == 1 and t.numel() == n and \
-            t.is_contiguous() and t.get_device() == device:
-        return t.data_ptr()
+    try:
+        if t.dtype is _INT32 and t.dim() == 1 and t.numel() == n and t.is_contiguous() and t.get_device() == device:
+            return t.data_ptr()
+    except AttributeError:
+        pass
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor, got {type(t).__name__}")
     raise ValueError(f"{name} must be a contiguous int32 [{n}] on cuda:{device}, got {list(t.shape)} {t.dtype} on {t.device}")
@@ -1036,11 +1041,9 @@ def _requests(t: torch.Tensor, name: str) -> tuple[int, int]:
 
 def _call_on(device: int, name: str, *args) -> None:
     """``_lib.call`` on the current stream of `device`, whichever device is current."""
-    if device != _current_device():
+    if device != _current_device() or _raw_stream is None:
         with torch.cuda.device(device):
             _lib.call(name, *args, _stream())
-    elif _raw_stream is None:
-        _lib.call(name, *args, _stream())
     else:
         _lib.call(name, *args, _raw_stream(device))
 
@@ -1062,7 +1065,10 @@ class PagedStep:
 
     @classmethod
     def empty(cls, requests: int, tokens: int, device) -> "PagedStep":
-        buf = torch.empty(3 * requests + 2 + 2 * tokens, dtype=torch.int32, device=device)
+        return cls._of(torch.empty(3 * requests + 2 + 2 * tokens, dtype=torch.int32, device=device), requests, tokens)
+
+    @classmethod
+    def _of(cls, buf: torch.Tensor, requests: int, tokens: int) -> "PagedStep":
         return cls(*buf.split_with_sizes((requests + 1, requests, 1, requests, tokens, tokens)))
 
 
@@ -1091,9 +1097,10 @@ def paged_step(lengths: torch.Tensor, new: torch.Tensor, block_table: torch.Tens
     if out is None:
         if tokens < 0:
             raise ValueError(f"tokens {tokens}")
-        out = PagedStep.empty(r, tokens, lengths.device)
-        ptrs = (out.starts.data_ptr(), out.lengths.data_ptr(), out.seq_lens.data_ptr(), out.positions.data_ptr(),
-                out.slots.data_ptr(), out.free_count.data_ptr())
+        buf = lengths.new_empty(3 * r + 2 + 2 * tokens)
+        out, first = PagedStep._of(buf, r, tokens), buf.data_ptr()
+        ptrs = (first, first + 4 * (r + 1), first + 4 * (2 * r + 2), first + 4 * (3 * r + 2),
+                first + 4 * (3 * r + 2 + tokens), first + 4 * (2 * r + 1))
     else:
         ptrs = [_index(getattr(out, name), "out." + name, n, dev) for name, n in (
             ("starts", r + 1), ("lengths", r), ("seq_lens", r), ("positions", tokens), ("slots", tokens), ("free_count", 1))]
@@ -1113,20 +1120,22 @@ def paged_trim(lengths: torch.Tensor, keep: torch.Tensor, block_table: torch.Ten
     at, to = _index(lengths, "lengths", r, dev), _index(keep, "keep", r, dev)
     free, had = _index(free_pages, "free_pages", pages, dev), _index(free_count, "free_count", 1, dev)
     table, stride, width = _table(block_table, r, dev)
-    kept, count = torch.empty(r + 1, dtype=torch.int32, device=lengths.device).split_with_sizes((r, 1))
+    kept, count = lengths.new_empty(r + 1).split_with_sizes((r, 1))
     _call_on(dev, "mosaic_paged_trim", at, to, table, stride, free, had, r, width, pages, page_size, kept.data_ptr(),
              count.data_ptr())
     return kept, count
 
 
+_CODES = (torch.uint8, torch.float8_e4m3fn)
+_SCALES = (torch.uint8, torch.float8_e8m0fnu)
+
+
 def _paged_cache(codes: torch.Tensor, scales: torch.Tensor, device: int) -> tuple:
     """codes [P, NB, Hkv, 2, 64 D] and scales [P, NB, Hkv, 2], read and written in place -> (P, NB, Hkv, D)."""
-    for t, name in ((codes, "codes"), (scales, "scales")):
-        if not isinstance(t, torch.Tensor):
-            raise TypeError(f"{name} must be a torch.Tensor, got {type(t).__name__}")
-    if codes.dim() == 5 and codes.dtype in (torch.uint8, torch.float8_e4m3fn) and codes.is_contiguous() and \
-            scales.dtype in (torch.uint8, torch.float8_e8m0fnu) and scales.is_contiguous() and \
-            codes.get_device() == device and scales.get_device() == device:
+    if not isinstance(codes, torch.Tensor) or not isinstance(scales, torch.Tensor):
+        raise TypeError(f"codes and scales must be torch.Tensors, got {type(codes).__name__} and {type(scales).__name__}")
+    if codes.dim() == 5 and codes.dtype in _CODES and codes.is_contiguous() and scales.dtype in _SCALES and \
+            scales.is_contiguous() and codes.get_device() == device and scales.get_device() == device:
         p, nb, hkv, two, size = codes.shape
         if two == 2 and size % PAGED_BLOCK == 0 and scales.shape == (p, nb, hkv, 2):
             return p, nb, hkv, size // PAGED_BLOCK
@@ -1204,12 +1213,12 @@ def paged_attention(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, 
     elif max_new < 1:
         raise ValueError(f"max_new {max_new}")
     if out is None:
-        out = torch.empty((t, hq, d), dtype=torch.bfloat16, device=q.device)
+        out = q.new_empty((t, hq, d))
     elif out.shape != q.shape or out.dtype is not torch.bfloat16 or not out.is_contiguous() or out.get_device() != dev:
         raise ValueError(f"out must be a contiguous bf16 {list(q.shape)} on {q.device}")
     nbytes = _lib.lib().mosaic_paged_attention_workspace_bytes(t, r, hq, hkv, d, nb, width, max_new)
-    ws = _workspace(workspace, nbytes, q.device)
+    ws = _workspace(workspace, nbytes, q.device) if nbytes else None
     _call_on(dev, "mosaic_paged_attention", q_at, q_tok, q_head, t, hq, codes.data_ptr(), scales.data_ptr(), p, nb, hkv,
              d, table, stride, width, first, seq, r, None if sink is None else sink.data_ptr(), window, max_new,
-             softmax_scale, out.data_ptr(), ws.data_ptr(), ws.numel())
+             softmax_scale, out.data_ptr(), None if ws is None else ws.data_ptr(), nbytes)
     return out

@@ -155,7 +155,7 @@ def _attn(**kw):
     (dict(tokens=1 << 21), "tokens"), (dict(blocks=0), "blocks"), (dict(pages=0), "pages"), (dict(window=-1), "window"), (dict(new=-1), "max_new"),
     (dict(scale=float("nan")), "finite"), (dict(scale=float("inf")), "finite"), (dict(qt=260), "16 bytes"),
     (dict(q=ctypes.c_void_p(4104)), "16 bytes"), (dict(out=ctypes.c_void_p(4104)), "16 bytes"),
-    (dict(scales=ctypes.c_void_p(4097)), "16 bytes"), (dict(width=200, stride=200, nws=1000), "workspace"), (dict(nws=31), "workspace"), (dict(out=None), "null"),
+    (dict(scales=ctypes.c_void_p(4097)), "16 bytes"), (dict(width=200, stride=200, nws=1000), "workspace"), (dict(width=200, stride=200, ws=None), "workspace"), (dict(out=None), "null"),
     (dict(stride=1), "tables")])
 def test_attention_refusals(kw, text):
     _refused("mosaic_paged_attention", _attn(**kw), text)
@@ -164,8 +164,8 @@ def test_attention_refusals(kw, text):
 def test_workspace_sizes():
     """A query for every kind of call, those without requests among them, and 0 for shapes that are refused."""
     size = _lib.lib().mosaic_paged_attention_workspace_bytes
-    assert size(5, 0, 64, 8, 128, 1, 4, 0) > 0 and size(0, 0, 64, 8, 128, 1, 4, 0) > 0
-    assert size(64, 64, 64, 8, 128, 1, 16, 1) < 1024 < size(64, 64, 64, 8, 128, 1, 17, 1)  # narrow tables are not cut
+    assert size(5, 0, 64, 8, 128, 1, 40, 0) > 0 and size(0, 0, 64, 8, 128, 1, 40, 0) > 0
+    assert size(64, 64, 64, 8, 128, 1, 16, 1) == 0 < size(64, 64, 64, 8, 128, 1, 17, 1)  # narrow tables are not cut
     assert size(4096, 1, 64, 8, 128, 1, 64, 0) == 0  # many uncut tiles of one request need none
     assert size(512, 1, 64, 8, 128, 1, 480, 0) > 1 << 20
     for bad in ((1, 1, 3, 2, 128, 1, 1, 0), (1, 1, 8, 8, 96, 1, 1, 0), (1 << 21, 1, 8, 8, 64, 1, 1, 0),
