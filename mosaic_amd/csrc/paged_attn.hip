@@ -190,9 +190,11 @@ __device__ __forceinline__ void clear_rest(const AttnArgs& a, int64_t thread, in
 }
 
 template <int D, int NW>
-__global__ void __launch_bounds__(64 * NW) paged_attn_rows_kernel(const AttnArgs a) {
+constexpr int kRowsLds = NW / 2 * D * 16 * 4;  // the halves' sums meet in fp32
+template <int D, int NW>
+__device__ __forceinline__ void rows_body(const AttnArgs& a, uint8_t* lds) {
   constexpr int DG = D / 64, DT = D / 16;
-  __shared__ __attribute__((aligned(16))) f32x4_t so[NW / 2][DT * 4 * 16];
+  auto so = reinterpret_cast<f32x4_t(*)[DT * 4 * 16]>(lds);  // [NW / 2]
   __shared__ float sm[NW][16], sl[NW][16];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, q = lane >> 4, c = lane & 15;
   const float scale = a.scale * a.sign;
@@ -432,6 +434,12 @@ __global__ void __launch_bounds__(64 * NW) paged_attn_rows_kernel(const AttnArgs
   }
 }
 
+template <int D, int NW>
+__global__ void __launch_bounds__(64 * NW) paged_attn_rows_kernel(const AttnArgs a) {
+  __shared__ __attribute__((aligned(16))) uint8_t lds[kRowsLds<D, NW>];
+  rows_body<D, NW>(a, lds);
+}
+
 // Adds up the pieces of a tile that was cut.  256 threads, in groups of D / 4 lanes
 // (four dims each).  Up to 16 pieces: a group a row, one piece after the other.
 // More (few rows over a long axis): the groups share a row's pieces and meet in LDS.
@@ -566,24 +574,27 @@ __device__ __forceinline__ void stage_ready() {
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
 
+template <int D>
+constexpr int kTileLds = 4 * 2 * kBlock * D;  // four stages
+// `group`: this workgroup's number among those of its kind, of `groups`
 template <int D, int NW>
-__global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) paged_attn_tile_kernel(const AttnArgs a) {
+__device__ __forceinline__ void tile_body(const AttnArgs& a, uint8_t* buf, int group, int groups) {
   constexpr int DG = D / 64, DQ = D / 32, ROWS = 32 * NW, STAGE = 2 * kBlock * D;
   constexpr int STAGES = 4, CPW = STAGE / 1024 / NW;  // copies of 1 KB a wave and block
   static_assert(CPW >= 1, "every wave copies");
-  __shared__ __attribute__((aligned(16))) uint8_t buf[STAGES * STAGE];
+  static_assert(kTileLds<D> == STAGES * STAGE, "the ring");
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int hl = lane >> 5, c = lane & 31, c16 = lane & 15, up = (lane >> 4) & 1;
 
-  if (a.zero_rows && blockIdx.y == 0) clear_rest<D>(a, (int64_t)blockIdx.x * 64 * NW + tid, (int64_t)gridDim.x * 64 * NW);
+  if (a.zero_rows && blockIdx.y == 0) clear_rest<D>(a, (int64_t)group * 64 * NW + tid, (int64_t)groups * 64 * NW);
   // the request and tile: key heads fastest (a head's workgroups meet in one XCD's
   // L2 where there are eight), the last tiles, which see most, first
-  const int h = blockIdx.x % a.hkv;
-  const uint32_t idx = blockIdx.x / a.hkv;
+  const int h = group % a.hkv;
+  const uint32_t idx = group / a.hkv;
   auto count = [&](const Request& x) { return many_rows(a, x) ? (uint32_t)((x.rows + ROWS - 1) / ROWS) : 0u; };
   const Place found = place<NW>(a, count, [](const Request&) { return 0u; },
                                 [&](uint32_t total) { return idx < total ? total - 1 - idx : total; });
-  if (gridDim.y > 1 && blockIdx.x == 0 && blockIdx.y == 0 && tid == 0) a.tile_info[0] = (int32_t)found.total;
+  if (gridDim.y > 1 && group == 0 && blockIdx.y == 0 && tid == 0) a.tile_info[0] = (int32_t)found.total;
   if (found.unit >= found.total) return;
   const uint32_t want = found.unit;
   const int r = found.r, tile = (int)(want - found.unit0);
@@ -946,6 +957,22 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) paged_attn_tile_ker
   }
 }
 
+template <int D, int NW>
+__global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) paged_attn_tile_kernel(const AttnArgs a) {
+  __shared__ __attribute__((aligned(16))) uint8_t lds[kTileLds<D>];
+  tile_body<D, NW>(a, lds, blockIdx.x, gridDim.x);
+}
+// Both kinds in one launch, the few-row workgroups first: a stream of the cache
+// beside products.
+template <int D, int NW>
+__global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) paged_attn_both_kernel(const AttnArgs a) {
+  __shared__ __attribute__((aligned(16))) uint8_t lds[kTileLds<D> > kRowsLds<D, NW> ? kTileLds<D> : kRowsLds<D, NW>];
+  if (blockIdx.x >= kGroups)
+    tile_body<D, NW>(a, lds, blockIdx.x - kGroups, gridDim.x - kGroups);
+  else if (blockIdx.y == 0)
+    rows_body<D, NW>(a, lds);
+}
+
 constexpr int kTileWaves = 4, kTileRows = 32 * kTileWaves;
 // Tiles of many rows are cut where there are fewer than this many, and into
 // pieces of no fewer blocks, by the width of the tables.
@@ -994,15 +1021,14 @@ Plan plan_of(int64_t tokens, int64_t requests, int64_t hq, int64_t hkv, int64_t 
 
 template <int D, int NW>
 int launch(const AttnArgs& a, const Plan& p, int few_rows, hipStream_t st) {
-  if (p.few) {
+  const unsigned tiles = (unsigned)(p.many_tiles * a.hkv), splits = (unsigned)p.splits;
+  if (p.few && p.many)
+    MOSAIC_LAUNCH((paged_attn_both_kernel<D, kTileWaves>), dim3(kGroups + tiles, splits), dim3(64 * kTileWaves), 0, st, a);
+  else if (p.few)
     MOSAIC_LAUNCH((paged_attn_rows_kernel<D, NW>), dim3(kGroups), dim3(64 * NW), 0, st, a);
-    MOSAIC_LAUNCH_CHECK("paged_attention");
-  }
-  if (p.many) {
-    MOSAIC_LAUNCH((paged_attn_tile_kernel<D, kTileWaves>), dim3((unsigned)(p.many_tiles * a.hkv), (unsigned)p.splits),
-                  dim3(64 * kTileWaves), 0, st, a);
-    MOSAIC_LAUNCH_CHECK("paged_attention");
-  }
+  else
+    MOSAIC_LAUNCH((paged_attn_tile_kernel<D, kTileWaves>), dim3(tiles, splits), dim3(64 * kTileWaves), 0, st, a);
+  MOSAIC_LAUNCH_CHECK("paged_attention");
   if (p.few && !p.whole) {
     // few tiles are cut into many pieces: a workgroup for each row of theirs
     const int z = p.few_tiles * a.hkv <= 64 ? few_rows : (few_rows * D + 1023) / 1024;
