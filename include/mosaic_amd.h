@@ -590,7 +590,8 @@ int mosaic_paged_kv_write(const uint16_t* k, const uint16_t* v, int64_t k_token_
  * exp(sink) to the softmax denominator.  out [tokens, q_heads, head_dim] bf16,
  * contiguous; rows without a key, and rows behind the last request, are zero.
  * max_new: the most rows of any request, or 0 if not known (it only sizes the
- * launch).  The workspace may be NULL where the query says 0 bytes. */
+ * launch).  starts ascends from 0 and out may not overlap q.  The workspace may be
+ * NULL where the query says 0 bytes. */
 size_t mosaic_paged_attention_workspace_bytes(int64_t tokens, int64_t requests, int64_t q_heads, int64_t kv_heads,
                                               int64_t head_dim, int64_t blocks, int64_t width, int64_t max_new);
 int mosaic_paged_attention(const uint16_t* q, int64_t q_token_stride, int64_t q_head_stride, int64_t tokens,

@@ -4,15 +4,16 @@
 //
 //   s = scale q . k in fp32 (k = code 2^(e - 127), exact in bf16), running
 //   maximum and sum of exp(s - m) in fp32, o = sum p v / (sum p + exp(sink - m)).
-//   p is rounded to bf16 for the matrix unit's value product (its sum is not):
-//   an error of at most 2^-9 a term, of either sign, against the 2^-9 of the
-//   bf16 output itself.
+//   p is rounded to bf16 for the matrix unit's value product: at most 2^-8 of a
+//   term, of either sign, as much as the bf16 output's own rounding.  Sums are
+//   fp32: of the unrounded p where rows are few, of the rounded (which makes the
+//   rounding's common part cancel) where they are many.
 //
 // Rows of one key head (tokens x query heads of its group) are tiled by 16.  A
 // work unit is a (request, key head, row tile, block of 64 tokens); the units of
 // all requests are numbered through and each workgroup takes an equal run of
 // them, so the lengths may be as unequal as they like.  A run's piece of one tile
-// is a segment: eight waves take its blocks in turn, keep (m, l, O) in registers
+// is a segment: the waves take its blocks in turn, keep (m, l, O) in registers
 // and meet in LDS at its end.  A tile in one segment is finished there; one that
 // is cut at a run's border leaves partial sums that paged_attn_join_kernel adds up.
 //
@@ -34,8 +35,8 @@ namespace {
 
 constexpr int kBlock = 64;
 constexpr int kRows = 16;           // rows of a tile
-// Workgroups of the few-row kernel: as many as are resident (eight waves a CU), so
-// that none begins late.  A context of 131000 tokens, 64 heads on 8 of 128: 58.5 us,
+// Workgroups of the few-row kernel: one a CU (eight waves; four beside the many-row
+// kernel's), so that none begins late.  A context of 131000 tokens, 64 heads on 8 of 128: 58.5 us,
 // with 512 62.6, with 1024 69.7; 64 requests of up to 32768: 386, 389 and 395 us.
 constexpr int kGroups = 256;
 constexpr int kWhole = 16;          // blocks of a table up to which tiles are not cut
@@ -57,6 +58,7 @@ struct AttnArgs {
   int r, tokens, hq, hkv, group, width, pages, nb, window;
   bool whole;      // few-row tiles are not cut (no join)
   int rows_max;    // requests of more rows are the many-row kernel's
+  uint32_t few_cap, many_cap;  // row tiles that the workspace and grid hold: ascending starts have no more
   bool zero_rows;  // the many-row kernel clears what lies behind the last request
   float scale;     // |softmax scale| log2(e)
   float sign;      // of the softmax scale
@@ -225,6 +227,7 @@ __device__ __forceinline__ void rows_body(const AttnArgs& a, uint8_t* lds) {
       after = request_of(a, ++r + 1);  // read ahead: the next segment does not wait for it
       tiles = (uint32_t)few_tiles(a, x);
       per = per_tile(x);
+      if (r >= a.r) return;  // only where starts that do not ascend number more units than 32 bits hold
     }
     // unit -> (head, tile, block), blocks fastest
     const uint32_t in = u - req0, ht = in / per;
@@ -393,7 +396,7 @@ __device__ __forceinline__ void rows_body(const AttnArgs& a, uint8_t* lds) {
     const bool whole = b_from == 0 && b_to == x.blocks;
     // a piece that begins inside its tile is its run's first, one that only ends inside is its last
     const int slot = 2 * (int)blockIdx.x + (b_from == 0 ? 1 : 0);
-    if (!a.whole && b_from == 0 && tid == 0) {  // the join's list: this tile's rows and the runs that hold it
+    if (!a.whole && b_from == 0 && (uint32_t)(tile0 + tile) < a.few_cap && tid == 0) {  // the join's list: this tile's rows and the runs that hold it
       int32_t* t = a.info + 8 + ((int64_t)(tile0 + tile) * a.hkv + h) * 8;
       t[0] = (x.s0 + row0 / a.group) * a.group + row0 % a.group;
       t[1] = rows;
@@ -593,7 +596,10 @@ __device__ __forceinline__ void tile_body(const AttnArgs& a, uint8_t* buf, int g
   const uint32_t idx = group / a.hkv;
   auto count = [&](const Request& x) { return many_rows(a, x) ? (uint32_t)((x.rows + ROWS - 1) / ROWS) : 0u; };
   const Place found = place<NW>(a, count, [](const Request&) { return 0u; },
-                                [&](uint32_t total) { return idx < total ? total - 1 - idx : total; });
+                                [&](uint32_t total) {
+                                  const uint32_t last = min(total, a.many_cap);
+                                  return idx < last ? last - 1 - idx : total;
+                                });
   if (gridDim.y > 1 && group == 0 && blockIdx.y == 0 && tid == 0) a.tile_info[0] = (int32_t)found.total;
   if (found.unit >= found.total) return;
   const uint32_t want = found.unit;
@@ -1091,10 +1097,13 @@ extern "C" int mosaic_paged_attention(const uint16_t* q, int64_t q_token_stride,
   const Plan p = plan_of(tokens, requests, q_heads, kv_heads, head_dim, width * blocks, max_new);
   MOSAIC_CHECK_ARG(p.total == 0 || (workspace && workspace_bytes >= (size_t)p.total), "paged_attention: workspace of %lld bytes, %lld needed",
                    (long long)workspace_bytes, (long long)p.total);
-  // the few-row kernel numbers its (tile, head, block) units in 32 bits
-  MOSAIC_CHECK_ARG(p.few_tiles * kv_heads < (1ll << 31) / (width * blocks) && p.many_tiles * kv_heads < (1ll << 31),
+  // the few-row kernel numbers its (tile, head, block) units in 32 bits, a launch its threads
+  MOSAIC_CHECK_ARG(p.few_tiles * kv_heads < (1ll << 31) / (width * blocks) &&
+                       (p.many_tiles * kv_heads + kGroups) * 64 * kTileWaves < (1ll << 32),
                    "paged_attention: %lld row tiles over tables of %lld blocks are too many for one call",
                    (long long)((p.few_tiles + p.many_tiles) * kv_heads), (long long)(width * blocks));
+  const uint16_t* q_end = q + (tokens - 1) * q_token_stride + (q_heads - 1) * q_head_stride + head_dim;
+  MOSAIC_CHECK_ARG(q_end <= out || out + tokens * q_heads * head_dim <= q, "paged_attention: out overlaps q");
   AttnArgs a{};
   a.q = q;
   a.codes = codes;
@@ -1112,6 +1121,8 @@ extern "C" int mosaic_paged_attention(const uint16_t* q, int64_t q_token_stride,
   a.tile_ml = (float*)(ws + p.tile_ml);
   a.tile_info = (int32_t*)(ws + p.tile_info);
   a.rows_max = p.rows_max;
+  a.few_cap = (uint32_t)p.few_tiles;
+  a.many_cap = (uint32_t)p.many_tiles;
   a.whole = p.whole;
   a.zero_rows = !p.few;
   a.q_tok = q_token_stride;

@@ -76,9 +76,10 @@ __global__ void __launch_bounds__(256) paged_step_kernel(const StepArgs a) {
     for (int i = 0; i < EACH; ++i) {
       const bool in = r0 + i < a.r;
       len[i] = in ? (uint32_t)max(a.lengths[r0 + i], 0) : 0u;
-      // a count past the token rows is as good as one more than they are: the sums stay in 32 bits
+      // a count past the token rows is as good as one more than they are, and so is a
+      // thread's sum: 256 of them stay in 32 bits
       n[i] = in ? min((uint32_t)max(a.add[r0 + i], 0), a.tokens + 1) : 0u;
-      sum_n += n[i];
+      sum_n = min(sum_n + n[i], a.tokens + 1);
     }
     uint32_t total, end[EACH], need[EACH], before[EACH];
     uint32_t sum = tok + block_excl_scan(sum_n, sums, total);

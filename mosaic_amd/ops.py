@@ -1023,7 +1023,7 @@ def _table(t: torch.Tensor, rows: int, device: int) -> tuple[int, int, int]:
         raise TypeError(f"block_table must be a torch.Tensor, got {type(t).__name__}")
     if t.dtype is torch.int32 and t.dim() == 2 and t.get_device() == device:
         (r, b), (stride, inner) = t.shape, t.stride()
-        if r == rows and b >= 1 and inner == 1 and (stride >= b or rows <= 1):
+        if r == rows and b >= 1 and (inner == 1 or b == 1 or rows == 0) and (stride >= b or rows <= 1):
             return t.data_ptr(), max(stride, b), b
     raise ValueError(f"block_table must be [{rows}, B] int32 with unit inner stride on cuda:{device}, got {list(t.shape)} "
                      f"{t.dtype} strides {t.stride()} on {t.device}")
@@ -1163,8 +1163,8 @@ def paged_kv_write(k: torch.Tensor, v: torch.Tensor, codes: torch.Tensor, scales
     """Write a step's keys and values k, v [T, Hkv, D] bf16 (D = 64, 128 or 256)
     into the paged cache, 8 bits a value: ``codes`` [P, NB, Hkv, 2, 64 D] e4m3 and
     ``scales`` [P, NB, Hkv, 2] e8m0, one scale a block of 64 tokens and head,
-    2^e with the largest magnitude at most 448 2^e.  ``starts`` and ``seq_lens`` as in
-    ``PagedStep``.  A block that held tokens before keeps its scale or moves to a
+    2^e with the largest magnitude at most 448 2^e.  ``starts`` (ascending from 0) and ``seq_lens`` as in
+    ``PagedStep``; no block that takes new tokens may be in two requests' tables.  A block that held tokens before keeps its scale or moves to a
     larger one; the rest of a block that begins here is zeroed."""
     (k, k_at, k_tok, k_head), (v, v_at, v_tok, v_head) = _paged_rows(k, "k"), _paged_rows(v, "v")
     dev = k.get_device()
@@ -1193,7 +1193,8 @@ def paged_attention(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, 
     Decode steps, drafts, pieces of prompts and whole prompts may share a call.
     Rows without a key and rows behind the last request are zero.  ``max_new``:
     the most rows of any request where the caller knows it (it only sizes the
-    launches).  A ``workspace`` serves one call at a time: calls on other
+    launches).  ``starts`` ascends from 0.  ``out`` may not overlap q.  Requests may
+    share pages (a common prefix).  A ``workspace`` serves one call at a time: calls on other
     streams, and graphs that may replay at once, need one each."""
     q, q_at, q_tok, q_head = _paged_rows(q, "q")
     dev = q.get_device()

@@ -148,8 +148,10 @@ def attention(q, codes, scales, table, starts, seq, scale, sink=None, window=0):
       sums   L u a term over the L keys
       range  an exponential below 2^-126, fp32's smallest normal number, may be taken as zero: at most
              2^-126 |v| a key, with l >= 1 (the key of the maximum)
+      a denominator that sums the rounded probabilities: o' - o = sum p d (v - o) / l' with |d| <= 2^-8,
+             so 2^-8 |o| beside the 2^-8 A of the numerator
     so |do| <= A (2^-8 + 2 (2 max|ds| + 2^-22 + L u)) + 2^-8 |o| with A = sum p |v| / l (the second
-    summand twice: numerator and denominator) and L 2^-126 max|v|, and the last rounding's 2^-8 of what it rounds."""
+    summand twice: numerator and denominator) and L 2^-126 max|v| and 2^-8 |o|, and the last rounding's 2^-8 of what it rounds."""
     t, hq, d = q.shape
     hkv = codes.shape[2]
     nb = codes.shape[1]
@@ -179,6 +181,7 @@ def attention(q, codes, scales, table, starts, seq, scale, sink=None, window=0):
                 ds = float(np.max((d + 2) * u * abs(scale) * (np.abs(kk) @ np.abs(q[j, h])) + 4 * u * np.abs(s)))
                 a = p @ np.abs(vv) / den
                 tol[j, h] = a * (2.0 ** -8 + 2 * (2 * ds + 2.0 ** -22 + see.size * u))
+                tol[j, h] += 2.0 ** -8 * np.abs(o[j, h])
                 tol[j, h] += see.size * 2.0 ** -126 * np.abs(vv).max(0)
                 tol[j, h] += 2.0 ** -8 * (np.abs(o[j, h]) + tol[j, h])
     return o, tol

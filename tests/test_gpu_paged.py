@@ -85,6 +85,21 @@ def test_step_rows_and_tables_that_do_not_suffice(dev):
         np.testing.assert_array_equal(t.cpu().numpy(), tb)
 
 
+@pytest.mark.parametrize("r", [2048, 2100, 4096])
+def test_step_counts_past_the_most_rows(dev, r):
+    """The most rows there may be, and counts whose sum passes 32 bits: after the first that does not fit, none does."""
+    from mosaic_amd import ops
+    lengths, new = np.zeros(r, np.int32), np.full(r, 2 ** 30, np.int32)
+    new[:3] = 5, 0, 7
+    table, free, count, _ = _pool(np.random.default_rng(6), lengths, lengths + 1, 64, 9)
+    tokens, t = 2 ** 21 - 1, _i32(table, dev)
+    s = ops.paged_step(_i32(lengths, dev), _i32(new, dev), t, tokens, 64, _i32(free, dev), _i32([count], dev))
+    want = P.step(lengths, new, table, tokens, 64, free, count)
+    for name, x in want.items():
+        np.testing.assert_array_equal(getattr(s, name).cpu().numpy(), x, err_msg=name)
+    np.testing.assert_array_equal(t.cpu().numpy(), table)
+
+
 def test_step_without_requests(dev):
     from mosaic_amd import ops
     s = ops.paged_step(_i32([], dev), _i32([], dev), torch.zeros(0, 3, dtype=torch.int32, device=dev), 5, 64,
@@ -353,6 +368,41 @@ def test_attention_unplaced_requests_give_zeros(dev):
                             _i32([0, 2, 3, 4], dev), _i32([0, 9, 0], dev), 0.125,
                             sink=torch.zeros(2, device=dev), out=out)
     assert not o[[0, 1, 3, 4, 5]].any() and o[2].abs().max() > 0
+
+
+@pytest.mark.parametrize("new", [[1, 2, 1], [90, 1, 40]])
+def test_attention_of_requests_that_share_a_prefix(dev, new):
+    def change(c, s, table, seq, starts):
+        table[1:, :3] = table[0, :3]
+    _attention_case(dev, np.random.default_rng(33), 8, 2, 128, 64, [200, 300, 192], new, change=change)
+
+
+def test_calls_without_rows(dev):
+    """A step in which every request rests: nothing is read or written."""
+    from mosaic_amd import ops
+    rng = np.random.default_rng(34)
+    c, s = _cache(rng, 4, 1, 2, 64)
+    ct, st = torch.from_numpy(c).to(dev), torch.from_numpy(s).to(dev)
+    x = torch.empty(0, 2, 64, dtype=torch.bfloat16, device=dev)
+    for r in (0, 3):
+        table, starts, seq = _i32(np.zeros((r, 2)), dev), _i32(np.zeros(r + 1), dev), _i32(np.full(r, 70), dev)
+        ops.paged_kv_write(x, x, ct, st, table, starts, seq)
+        assert ops.paged_attention(x, ct, st, table, starts, seq, 0.125).shape == (0, 2, 64)
+    np.testing.assert_array_equal(ct.cpu().numpy(), c)
+    np.testing.assert_array_equal(st.cpu().numpy(), s)
+
+
+def test_tables_of_one_page(dev):
+    """A column of a table turned on its side: the stride within a row of one entry does not matter."""
+    from mosaic_amd import ops
+    rng = np.random.default_rng(35)
+    c, s = (torch.from_numpy(x).to(dev) for x in _cache(rng, 4, 1, 2, 64))
+    q = torch.from_numpy(_bf16(rng, 3, 2, 64)).to(dev).to(torch.bfloat16)
+    table, starts, seq = _i32([[2], [0], [3]], dev), _i32([0, 1, 2, 3], dev), _i32([5, 64, 1], dev)
+    want = ops.paged_attention(q, c, s, table, starts, seq, 0.125)
+    turned = _i32([[2, 0, 3]], dev).t()
+    assert turned.stride() == (1, 3)
+    assert torch.equal(ops.paged_attention(q, c, s, turned, starts, seq, 0.125), want)
 
 
 def test_attention_without_requests_clears_its_rows(dev):

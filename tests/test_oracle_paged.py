@@ -156,7 +156,8 @@ def _attn(**kw):
     (dict(scale=float("nan")), "finite"), (dict(scale=float("inf")), "finite"), (dict(qt=260), "16 bytes"),
     (dict(q=ctypes.c_void_p(4104)), "16 bytes"), (dict(out=ctypes.c_void_p(4104)), "16 bytes"),
     (dict(scales=ctypes.c_void_p(4097)), "16 bytes"), (dict(width=200, stride=200, nws=1000), "workspace"), (dict(width=200, stride=200, ws=None), "workspace"), (dict(out=None), "null"),
-    (dict(stride=1), "tables")])
+    (dict(stride=1), "tables"), (dict(), "overlaps"),
+    (dict(tokens=1 << 20, r=1 << 20, hq=16, hkv=16), "too many")])
 def test_attention_refusals(kw, text):
     _refused("mosaic_paged_attention", _attn(**kw), text)
 
