@@ -10,9 +10,10 @@
 //   rounding's common part cancel) where they are many.
 //
 // Rows of one key head (tokens x query heads of its group) are tiled by 16.  A
-// work unit is a (request, key head, row tile, block of 64 tokens); the units of
-// all requests are numbered through and each workgroup takes an equal run of
-// them, so the lengths may be as unequal as they like.  A run's piece of one tile
+// work unit is a (request, key head, row tile, block of 64 tokens), and a tile's
+// first block is preceded by kStart empty ones; the units of all requests are
+// numbered through and each workgroup takes an equal run of them, so the lengths
+// may be as unequal as they like.  A run's piece of one tile
 // is a segment: the waves take its blocks in turn, keep (m, l, O) in registers
 // and meet in LDS at its end.  A tile in one segment is finished there; one that
 // is cut at a run's border leaves partial sums that paged_attn_join_kernel adds up.
@@ -39,7 +40,15 @@ constexpr int kRows = 16;           // rows of a tile
 // kernel's), so that none begins late.  A context of 131000 tokens, 64 heads on 8 of 128: 58.5 us,
 // with 512 62.6, with 1024 69.7; 64 requests of up to 32768: 386, 389 and 395 us.
 constexpr int kGroups = 256;
-constexpr int kWhole = 16;          // blocks of a table up to which tiles are not cut
+// What a tile's first piece costs beside its blocks, in blocks (its queries, the chain of page, codes
+// and scores, the meeting of the waves): a run of many short tiles gets as much less.  64 requests
+// of up to 2000 tokens, 64 heads on 8 of 128: 61.0 us without, 41.5 with 4, 34.6 with 8, 33.0 with
+// 14; 64 of up to 32768: 387, 376, 368, 368; 8 pieces beside them 46.4, 44.9, 45.7, 47.2.
+constexpr int kStart = 8;
+// Blocks of a table up to which tiles are not cut, which saves the join: a tile is then the run's
+// that holds its first unit.  Tables of 30 blocks, 64 heads on 8 of 128, cut and whole: 1 request 13.4 and
+// 12.6 us, 16 17.3 and 13.9, 64 31.2 and 28.4, 200 90.1 and 87.2; of 50: 12.8 and 17.8, 19.8 and 20.5, 50.7 and 55.6.
+constexpr int kWhole = 32;
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct AttnArgs {
@@ -201,8 +210,8 @@ __device__ __forceinline__ void rows_body(const AttnArgs& a, uint8_t* lds) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, q = lane >> 4, c = lane & 15;
   const float scale = a.scale * a.sign;
 
-  // units of a tile and head: its blocks, or the tile as a whole
-  auto per_tile = [&](const Request& x) { return a.whole ? 1u : (uint32_t)x.blocks; };
+  // units of a tile and head: what it costs.  Where tiles are whole, they are their first unit's run's.
+  auto per_tile = [&](const Request& x) { return (uint32_t)(kStart + x.blocks); };
   uint32_t share = 0;
   const Place at = place<NW>(
       a, [&](const Request& x) { return (uint32_t)few_tiles(a, x) * (uint32_t)a.hkv * per_tile(x); },
@@ -231,10 +240,12 @@ __device__ __forceinline__ void rows_body(const AttnArgs& a, uint8_t* lds) {
     }
     // unit -> (head, tile, block), blocks fastest
     const uint32_t in = u - req0, ht = in / per;
-    const int b_from = a.whole ? 0 : (int)(in % per), b_to = a.whole ? x.blocks : (int)min(per, (uint32_t)b_from + (u1 - u));
+    const int begin = (int)(in % per), units = (int)(a.whole ? per - begin : min(per - begin, u1 - u));
+    const int b_from = a.whole ? 0 : max(begin - kStart, 0), b_to = begin + units - kStart;
     const int h = (int)(ht / tiles), tile = (int)(ht % tiles);
-    const uint32_t tile_u0 = u - b_from;
-    u += a.whole ? 1 : b_to - b_from;
+    const uint32_t tile_u0 = u - begin;
+    u += units;
+    if (a.whole ? begin > 0 : b_to <= 0) continue;  // an earlier run's; the run ends before the tile's first block
     const int row0 = tile * kRows, rows = min(kRows, x.rows - row0);
     const int row = row0 + min(c, rows - 1);
     const int tok = row / a.group, head = h * a.group + row % a.group;
@@ -400,7 +411,7 @@ __device__ __forceinline__ void rows_body(const AttnArgs& a, uint8_t* lds) {
       int32_t* t = a.info + 8 + ((int64_t)(tile0 + tile) * a.hkv + h) * 8;
       t[0] = (x.s0 + row0 / a.group) * a.group + row0 % a.group;
       t[1] = rows;
-      t[2] = (int)((tile_u0 + x.blocks - 1) / share - blockIdx.x) + 1;
+      t[2] = (int)((tile_u0 + per - 1) / share - blockIdx.x) + 1;
       t[3] = slot;
       t[4] = slot + 1;
       t[5] = 2;
@@ -1001,7 +1012,6 @@ Plan plan_of(int64_t tokens, int64_t requests, int64_t hq, int64_t hkv, int64_t 
   p.many = some > 0 && most > kRows;
   p.few = !p.many || requests > 1;
   p.rows_max = !p.many ? INT_MAX : p.few ? kRows : 0;
-  // a table of few blocks: its tiles are a turn or two of a workgroup's waves, less than a join takes
   p.whole = width_blocks <= kWhole;
   p.few_tiles = p.few ? (p.many ? some : tokens * group / kRows + some) : 0;
   p.many_tiles = p.many ? tokens * group / kTileRows + some : 0;
@@ -1098,7 +1108,7 @@ extern "C" int mosaic_paged_attention(const uint16_t* q, int64_t q_token_stride,
   MOSAIC_CHECK_ARG(p.total == 0 || (workspace && workspace_bytes >= (size_t)p.total), "paged_attention: workspace of %lld bytes, %lld needed",
                    (long long)workspace_bytes, (long long)p.total);
   // the few-row kernel numbers its (tile, head, block) units in 32 bits, a launch its threads
-  MOSAIC_CHECK_ARG(p.few_tiles * kv_heads < (1ll << 31) / (width * blocks) &&
+  MOSAIC_CHECK_ARG(p.few_tiles * kv_heads < (1ll << 31) / (kStart + width * blocks) &&
                        (p.many_tiles * kv_heads + kGroups) * 64 * kTileWaves < (1ll << 32),
                    "paged_attention: %lld row tiles over tables of %lld blocks are too many for one call",
                    (long long)((p.few_tiles + p.many_tiles) * kv_heads), (long long)(width * blocks));

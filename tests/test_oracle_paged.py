@@ -166,7 +166,7 @@ def test_workspace_sizes():
     """A query for every kind of call, those without requests among them, and 0 for shapes that are refused."""
     size = _lib.lib().mosaic_paged_attention_workspace_bytes
     assert size(5, 0, 64, 8, 128, 1, 40, 0) > 0 and size(0, 0, 64, 8, 128, 1, 40, 0) > 0
-    assert size(64, 64, 64, 8, 128, 1, 16, 1) == 0 < size(64, 64, 64, 8, 128, 1, 17, 1)  # narrow tables are not cut
+    assert size(64, 64, 64, 8, 128, 1, 32, 1) == 0 < size(64, 64, 64, 8, 128, 1, 33, 1)  # narrow tables are not cut
     assert size(4096, 1, 64, 8, 128, 1, 64, 0) == 0  # many uncut tiles of one request need none
     assert size(512, 1, 64, 8, 128, 1, 480, 0) > 1 << 20
     for bad in ((1, 1, 3, 2, 128, 1, 1, 0), (1, 1, 8, 8, 96, 1, 1, 0), (1 << 21, 1, 8, 8, 64, 1, 1, 0),
