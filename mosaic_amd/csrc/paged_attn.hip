@@ -49,6 +49,11 @@ constexpr int kStart = 8;
 // that holds its first unit.  Tables of 30 blocks, 64 heads on 8 of 128, cut and whole: 1 request 13.4 and
 // 12.6 us, 16 17.3 and 13.9, 64 31.2 and 28.4, 200 90.1 and 87.2; of 50: 12.8 and 17.8, 19.8 and 20.5, 50.7 and 55.6.
 constexpr int kWhole = 32;
+// Up to this, where there are more tiles than workgroups, a tile is four waves' and a CU has two
+// workgroups, whose chains overlap.  64 heads on 8 of 128, eight and four waves: 256 requests of up to 500
+// tokens 56.5 and 42.2 us, 64 of up to 800 20.4 and 19.8, but 64 of up to 1700 28.4 and 29.1; with fewer
+// tiles, 16 of up to 800, 10.9 and 13.2.
+constexpr int kNarrow = 16;
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct AttnArgs {
@@ -203,7 +208,7 @@ __device__ __forceinline__ void clear_rest(const AttnArgs& a, int64_t thread, in
 template <int D, int NW>
 constexpr int kRowsLds = NW / 2 * D * 16 * 4;  // the halves' sums meet in fp32
 template <int D, int NW>
-__device__ __forceinline__ void rows_body(const AttnArgs& a, uint8_t* lds) {
+__device__ __forceinline__ void rows_body(const AttnArgs& a, uint8_t* lds, uint32_t groups) {
   constexpr int DG = D / 64, DT = D / 16;
   auto so = reinterpret_cast<f32x4_t(*)[DT * 4 * 16]>(lds);  // [NW / 2]
   __shared__ float sm[NW][16], sl[NW][16];
@@ -217,11 +222,11 @@ __device__ __forceinline__ void rows_body(const AttnArgs& a, uint8_t* lds) {
       a, [&](const Request& x) { return (uint32_t)few_tiles(a, x) * (uint32_t)a.hkv * per_tile(x); },
       [&](const Request& x) { return (uint32_t)few_tiles(a, x); },
       [&](uint32_t total) {
-        share = (total + kGroups - 1) / kGroups;
+        share = (total + groups - 1) / groups;
         if (!a.whole) share = max(share, (uint32_t)NW / 2);
         return min(blockIdx.x * (uint64_t)share, (uint64_t)total);
       });
-  clear_rest<D>(a, (int64_t)blockIdx.x * 64 * NW + tid, (int64_t)kGroups * 64 * NW);
+  clear_rest<D>(a, (int64_t)blockIdx.x * 64 * NW + tid, (int64_t)groups * 64 * NW);
   if (!a.whole && blockIdx.x == 0 && tid == 0) a.info[0] = (int32_t)at.tiles;
   const uint32_t u0 = at.unit, u1 = min(u0 + share, at.total);
   if (u0 >= at.total) return;
@@ -449,9 +454,9 @@ __device__ __forceinline__ void rows_body(const AttnArgs& a, uint8_t* lds) {
 }
 
 template <int D, int NW>
-__global__ void __launch_bounds__(64 * NW) paged_attn_rows_kernel(const AttnArgs a) {
+__global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) paged_attn_rows_kernel(const AttnArgs a) {
   __shared__ __attribute__((aligned(16))) uint8_t lds[kRowsLds<D, NW>];
-  rows_body<D, NW>(a, lds);
+  rows_body<D, NW>(a, lds, gridDim.x);
 }
 
 // Adds up the pieces of a tile that was cut.  256 threads, in groups of D / 4 lanes
@@ -987,7 +992,7 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) paged_attn_both_ker
   if (blockIdx.x >= kGroups)
     tile_body<D, NW>(a, lds, blockIdx.x - kGroups, gridDim.x - kGroups);
   else if (blockIdx.y == 0)
-    rows_body<D, NW>(a, lds);
+    rows_body<D, NW>(a, lds, kGroups);
 }
 
 constexpr int kTileWaves = 4, kTileRows = 32 * kTileWaves;
@@ -998,7 +1003,7 @@ constexpr int kSplitGroups = 512, kSplitBlocks = 32;
 // How a call is carried out, by its sizes alone (the lengths are on the GPU).
 struct Plan {
   bool few, many;      // which kernels run
-  bool whole;          // few-row tiles are not cut
+  bool whole, narrow;  // few-row tiles are not cut; two workgroups a CU share the work
   int rows_max;        // requests of up to so many rows are the few-row kernel's
   int64_t few_tiles, many_tiles, splits;  // bounds of the tiles a head; splits: workgroups a many-row tile
   int64_t o, ml, info, tile_o, tile_ml, tile_info, total;  // workspace
@@ -1023,6 +1028,7 @@ Plan plan_of(int64_t tokens, int64_t requests, int64_t hq, int64_t hkv, int64_t 
     if (p.splits > 16) p.splits = 16;
     if (p.splits < 1) p.splits = 1;
   }
+  p.narrow = p.few && !p.many && width_blocks <= kNarrow && p.few_tiles * hkv > kGroups;
   const int64_t slots = p.few && !p.whole ? 2 * kGroups : 0;
   const int64_t tile_slots = p.splits > 1 ? p.many_tiles * hkv * p.splits * (kTileRows / kRows) : 0;
   p.o = 0;
@@ -1040,6 +1046,8 @@ int launch(const AttnArgs& a, const Plan& p, int few_rows, hipStream_t st) {
   const unsigned tiles = (unsigned)(p.many_tiles * a.hkv), splits = (unsigned)p.splits;
   if (p.few && p.many)
     MOSAIC_LAUNCH((paged_attn_both_kernel<D, kTileWaves>), dim3(kGroups + tiles, splits), dim3(64 * kTileWaves), 0, st, a);
+  else if (p.few && p.narrow)
+    MOSAIC_LAUNCH((paged_attn_rows_kernel<D, 4>), dim3(NW / 4 * kGroups), dim3(256), 0, st, a);
   else if (p.few)
     MOSAIC_LAUNCH((paged_attn_rows_kernel<D, NW>), dim3(kGroups), dim3(64 * NW), 0, st, a);
   else

@@ -312,6 +312,14 @@ def test_attention_many_short_requests(dev):
     _attention_case(dev, rng, 4, 1, 64, 64, held, rng.integers(0, 3, 700), pad=2)
 
 
+@pytest.mark.parametrize("hq,hkv,d,r,most,window", [(8, 8, 128, 40, 700, 0), (16, 8, 64, 70, 900, 100), (6, 6, 256, 50, 300, 0),
+                                                     (16, 4, 128, 70, 1500, 0), (16, 4, 128, 30, 2500, 600)])
+def test_attention_more_tiles_than_workgroups(dev, hq, hkv, d, r, most, window):
+    """Whole and cut tiles, several of a workgroup's, of unequal lengths; resting requests and drafts among them."""
+    rng = np.random.default_rng(36 + r)
+    _attention_case(dev, rng, hq, hkv, d, 64, rng.integers(0, most, r), rng.integers(0, 4, r), window, sink=True, max_new=3, pad=2)
+
+
 def test_attention_scale_bytes(dev):
     """The least and largest scales that the writer makes of bf16 values near its range's ends, mixed in one row."""
     def change(c, s, table, seq, starts):
