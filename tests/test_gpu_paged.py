@@ -272,7 +272,7 @@ def test_attention_long_context(dev):
 
 @pytest.mark.parametrize("hq,hkv,d,page,held,new,window", [
     (8, 1, 128, 64, [3000, 40, 0], [100, 1, 17], 0), (16, 2, 64, 128, [5000], [60], 0), (4, 4, 256, 64, [2000], [33], 0),
-    (6, 2, 128, 64, [1500, 1500], [40, 90], 700), (16, 1, 64, 64, [4000], [2], 0)])
+    (6, 2, 128, 64, [1500, 1500], [40, 90], 700), (16, 1, 64, 64, [4000], [2], 0), (4, 1, 64, 64, [4000], [260], 2000)])
 def test_attention_pieces_behind_long_contexts(dev, hq, hkv, d, page, held, new, window):
     """Few tiles of many rows over a long axis: each is cut among workgroups and joined."""
     _attention_case(dev, np.random.default_rng(d + len(held)), hq, hkv, d, page, held, new, window, sink=True)
