@@ -412,7 +412,8 @@ __device__ __forceinline__ void rows_body(const AttnArgs& a, uint8_t* lds, uint3
     const bool whole = b_from == 0 && b_to == x.blocks;
     // a piece that begins inside its tile is its run's first, one that only ends inside is its last
     const int slot = 2 * (int)blockIdx.x + (b_from == 0 ? 1 : 0);
-    if (!a.whole && b_from == 0 && (uint32_t)(tile0 + tile) < a.few_cap && tid == 0) {  // the join's list: this tile's rows and the runs that hold it
+    // the join's list: this tile's rows and the runs that hold it
+    if (!a.whole && b_from == 0 && (uint32_t)(tile0 + tile) < a.few_cap && tid == 0) {
       int32_t* t = a.info + 8 + ((int64_t)(tile0 + tile) * a.hkv + h) * 8;
       t[0] = (x.s0 + row0 / a.group) * a.group + row0 % a.group;
       t[1] = rows;
@@ -1119,7 +1120,8 @@ extern "C" int mosaic_paged_attention(const uint16_t* q, int64_t q_token_stride,
                        (uintptr_t)scales % 2 == 0 && q_token_stride % 8 == 0 && q_head_stride % 8 == 0,
                    "paged_attention: q, out, codes and the workspace are read and written 16 bytes at a time");
   const Plan p = plan_of(tokens, requests, q_heads, kv_heads, head_dim, width * blocks, max_new, window);
-  MOSAIC_CHECK_ARG(p.total == 0 || (workspace && workspace_bytes >= (size_t)p.total), "paged_attention: workspace of %lld bytes, %lld needed",
+  MOSAIC_CHECK_ARG(p.total == 0 || (workspace && workspace_bytes >= (size_t)p.total),
+                   "paged_attention: workspace of %lld bytes, %lld needed",
                    (long long)workspace_bytes, (long long)p.total);
   // the few-row kernel numbers its (tile, head, block) units in 32 bits, a launch its threads
   MOSAIC_CHECK_ARG(p.few_tiles * kv_heads < (1ll << 31) / (kStart + width * blocks) &&

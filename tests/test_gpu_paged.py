@@ -290,7 +290,7 @@ def test_attention_scales(dev, scale):
 
 
 def test_attention_queries_of_unequal_size(dev):
-    """Rows from 2^-60 to 2^20 of the others, dims within a row over 2^16, rows of zeros: q in two e4m3 parts."""
+    """Rows from 2^-60 to 2^20 of the others, dims within a row over 2^16, rows of zeros."""
     from mosaic_amd import ops
     rng = np.random.default_rng(32)
     table, total, starts, seq = _batch(rng, [70], [60], 64)
