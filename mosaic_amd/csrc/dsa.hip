@@ -1215,18 +1215,20 @@ __device__ __forceinline__ uint32_t mla_lds_addr(const void* p) {
 // one 16-byte (resp. 4-byte) global -> LDS copy per lane; the LDS address of
 // lane i is base + 16 i (resp. 4 i).  Issued from inline asm so the compiler
 // neither waits for them before LDS reads nor stages them in registers; the
-// kernel waits with explicit vmcnt counts.
+// kernel waits with explicit vmcnt counts.  There has to be one wait state between
+// writing m0 and a load that takes it, which neither the hardware nor (inside an
+// asm text) the compiler sees to: the s_nop.
 __device__ __forceinline__ void mla_copy16(const void* g, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(__builtin_amdgcn_readfirstlane(lds)),
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(__builtin_amdgcn_readfirstlane(lds)),
                "v"(g) : "memory", "m0");
 }
 // the same from a wave-uniform base plus this lane's byte offset
 __device__ __forceinline__ void mla_copy16_s(const void* base, int off, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane(lds)),
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane(lds)),
                "v"(off), "s"(base) : "memory", "m0");
 }
 __device__ __forceinline__ void mla_copy4(const void* g, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, off" ::"s"(__builtin_amdgcn_readfirstlane(lds)),
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(__builtin_amdgcn_readfirstlane(lds)),
                "v"(g) : "memory", "m0");
 }
 

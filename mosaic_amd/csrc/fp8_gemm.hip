@@ -352,13 +352,14 @@ __device__ __forceinline__ uint32_t fp8_lds_addr(const void* p) {
   return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p;
 }
 // one 16-byte (resp. 4-byte) global -> LDS copy per lane; the LDS address of
-// lane i is base + 16 i (resp. 4 i)
+// lane i is base + 16 i (resp. 4 i).  s_nop: a load that takes m0 needs one wait
+// state behind its write, which nothing adds inside an asm text.
 __device__ __forceinline__ void fp8_copy16(const void* g, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(__builtin_amdgcn_readfirstlane(lds)),
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(__builtin_amdgcn_readfirstlane(lds)),
                "v"(g) : "memory", "m0");
 }
 __device__ __forceinline__ void fp8_copy4(const void* g, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, off" ::"s"(__builtin_amdgcn_readfirstlane(lds)),
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(__builtin_amdgcn_readfirstlane(lds)),
                "v"(g) : "memory", "m0");
 }
 
@@ -849,12 +850,13 @@ __device__ __forceinline__ int fp8_big_slot_row(int s) {
   return (s & ~127) + (t & 7) * 16 + (t >> 3);
 }
 
+// (s_nop: as in fp8_copy16)
 __device__ __forceinline__ void fp8_copy16_so(const void* base, uint32_t off, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane(lds)),
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane(lds)),
                "v"(off), "s"(base) : "memory", "m0");
 }
 __device__ __forceinline__ void fp8_copy4_so(const void* base, uint32_t off, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, %2" ::"s"(__builtin_amdgcn_readfirstlane(lds)),
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(__builtin_amdgcn_readfirstlane(lds)),
                "v"(off), "s"(base) : "memory", "m0");
 }
 

@@ -148,9 +148,11 @@ constexpr int kW8LA = 3, kW8DA = kW8LA + 1, kW8LB = 8;
 __device__ __forceinline__ uint32_t w8_lds_addr(const void* p) {
   return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p;
 }
-// one 16-byte global -> LDS copy per lane; the LDS address of lane i is base + 16 i
+// one 16-byte global -> LDS copy per lane; the LDS address of lane i is base + 16 i.
+// s_nop: a load that takes m0 needs one wait state behind its write, which nothing
+// adds inside an asm text.
 __device__ __forceinline__ void w8_copy16(const void* g, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(__builtin_amdgcn_readfirstlane(lds)),
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(__builtin_amdgcn_readfirstlane(lds)),
                "v"(g) : "memory", "m0");
 }
 

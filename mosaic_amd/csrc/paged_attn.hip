@@ -568,11 +568,12 @@ __device__ __forceinline__ float half_sum(float x) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 // run I of 1 KB, 16 bytes a lane, of those from g (one address for the wave) to LDS;
-// the immediate offset counts on both sides
+// the immediate offset counts on both sides.  s_nop: a load that takes m0 needs one
+// wait state behind its write, which nothing adds inside an asm text
 template <int I>
 __device__ __forceinline__ void lds_copy(const uint8_t* g, uint32_t lane16, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2 offset:%3" ::"s"(lds + I / 4 * 4096), "v"(lane16),
-               "s"(g + I / 4 * 4096), "n"(I % 4 * 1024)
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 offset:%3" ::"s"(lds + I / 4 * 4096),
+               "v"(lane16), "s"(g + I / 4 * 4096), "n"(I % 4 * 1024)
                : "memory", "m0");
 }
 // f(std::integral_constant<int, 0>) .. f(<N - 1>)

@@ -53,3 +53,20 @@ def test_mla_whole_split_q_wait(code_objects):
         between = ins[last + 1:wait]
         assert not any(x.startswith(("s_cbranch", "s_branch")) for x in between), sym
         assert sum(x.startswith("global_load") for x in between) >= left > 0, sym
+
+
+def test_copies_into_lds_wait_for_m0(code_objects):
+    """A copy into LDS takes its address from m0 and needs one wait state behind the write of m0, which the
+    hardware does not add: something else, or an s_nop, stands between them in every kernel."""
+    copies = 0
+    for obj in code_objects:
+        asm = subprocess.run([LLVM / "llvm-objdump", "-d", "--no-show-raw-insn", obj], check=True, capture_output=True,
+                             text=True).stdout
+        before = ""
+        for ln in asm.splitlines():
+            ins = ln.split("//")[0].strip() if ln.startswith("\t") else ""
+            if re.match(r"(global|buffer|scratch)_load_lds_|buffer_load_.*\blds$", ins):
+                copies += 1
+                assert not re.match(r"\S+ m0\b", before), (obj.name, before, ins)
+            before = ins or before
+    assert copies > 1000
