@@ -561,7 +561,7 @@ int mosaic_paged_step(const int32_t* lengths, const int32_t* add, int32_t* block
 /* Shortens requests to keep[r] tokens (0 releases one; more than it holds
  * changes nothing) and pushes the pages behind them, the last request's last
  * page first: the inverse of a step.  `pages` is the stack's capacity; the
- * tables are left as they are.  lengths_out and count_out may not overlap the
+ * tables, of fewer than 2^31 entries, are left as they are.  lengths_out and count_out may not overlap the
  * inputs (free_pages is updated in place). */
 int mosaic_paged_trim(const int32_t* lengths, const int32_t* keep, const int32_t* block_table, int64_t table_stride,
                       int32_t* free_pages, const int32_t* free_count, int64_t requests, int64_t width, int64_t pages,

@@ -505,6 +505,9 @@ extern "C" int mosaic_paged_trim(const int32_t* lengths, const int32_t* keep, co
   MOSAIC_CHECK_ARG(width >= 1 && width * page_size < (1ll << 30) && table_stride >= width,
                    "paged_trim: tables of %lld pages (rows hold fewer than 2^30 tokens)", (long long)width);
   MOSAIC_CHECK_ARG(pages >= 0 && pages * page_size < (1ll << 31), "paged_trim: %lld pages", (long long)pages);
+  // what lengths may say to hold in all is counted in 32 bits, and columns are found by that count
+  MOSAIC_CHECK_ARG(requests * width < (1ll << 31), "paged_trim: tables of %lld entries (below 2^31)",
+                   (long long)(requests * width));
   MOSAIC_CHECK_ARG(free_count && count_out && (pages == 0 || free_pages) &&
                        (requests == 0 || (lengths && keep && block_table && lengths_out)),
                    "paged_trim: null pointer");

@@ -197,3 +197,9 @@ def test_wrappers_refuse_cpu_tensors_and_bad_caches():
     for kw in (dict(page_size=32), dict(head_dim=96), dict(pages=0), dict(max_length=0)):
         with pytest.raises(ValueError):
             PagedKVCache(**{**dict(pages=4, kv_heads=1, head_dim=64, max_requests=1, max_length=64, device="cpu"), **kw})
+
+
+@pytest.mark.parametrize("r,width", [(1 << 12, 1 << 19), (1 << 20, 1 << 11), (1 << 8, (1 << 24) - 1)])
+def test_trim_refuses_tables_whose_pages_pass_32_bits(r, width):
+    """Lengths that claim whole tables would make the count of freed pages wrap, and columns be read outside a row."""
+    _refused("mosaic_paged_trim", _trim(r=r, width=width, stride=width), "entries")
