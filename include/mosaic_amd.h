@@ -588,7 +588,8 @@ int mosaic_paged_kv_write(const uint16_t* k, const uint16_t* v, int64_t k_token_
  * head_dim] bf16 (strides in elements, multiples of 8; 16-byte aligned), query
  * head h reads key head h / (q_heads / kv_heads); sink [q_heads] f32 or NULL adds
  * exp(sink) to the softmax denominator.  out [tokens, q_heads, head_dim] bf16,
- * contiguous; rows without a key, and rows behind the last request, are zero.
+ * contiguous; rows without a key, and rows behind the last request, are zero, and
+ * rows whose keys' scores are all -inf are 0 / 0 without a sink and 0 with one.
  * max_new: the most rows of any request, or 0 if not known (it only sizes the
  * launch).  starts ascends from 0 and out may not overlap q.  The workspace may be
  * NULL where the query says 0 bytes. */

@@ -7,7 +7,8 @@
 //   p is rounded to bf16 for the matrix unit's value product: at most 2^-8 of a
 //   term, of either sign, as much as the bf16 output's own rounding.  Sums are
 //   fp32: of the unrounded p where rows are few, of the rounded (which makes the
-//   rounding's common part cancel) where they are many.
+//   rounding's common part cancel) where they are many.  m begins at fp32's lowest
+//   number: a score of -inf, masked or overflowed, weighs 0 against it.
 //
 // Rows of one key head (tokens x query heads of its group) are tiled by 16.  A
 // work unit is a (request, key head, row tile, block of 64 tokens), and a tile's
@@ -55,6 +56,10 @@ constexpr int kWhole = 32;
 // tiles, 16 of up to 800, 10.9 and 13.2.
 constexpr int kNarrow = 16;
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLowest = -3.402823466e38f;  // fp32's: a maximum of nothing
+// Each block that a row sees a key of adds so much to its sum (1 and more where there is a
+// weight, which that does not round), so that a row of nothing but scores of -inf is told from one without keys
+constexpr float kSeen = 0x1p-100f, kWeightless = 0x1p-60f;
 
 struct AttnArgs {
   const uint16_t* q;
@@ -100,6 +105,15 @@ __device__ __forceinline__ int few_tiles(const AttnArgs& a, const Request& x) {
   return x.rows > a.rows_max ? 0 : (x.rows + kRows - 1) / kRows;
 }
 __device__ __forceinline__ bool many_rows(const AttnArgs& a, const Request& x) { return x.rows > a.rows_max; }
+
+// 1 / (l + exp2(sink - m)): what a row's sums are multiplied by.  Without weights they
+// are zeros, and so is the output: 0 / exp(sink), or by convention where the row sees
+// no key at all; but 0 / 0, not a number, where it sees some and has no sink.
+__device__ __forceinline__ float row_factor(const AttnArgs& a, int head, float m, float l) {
+  const float s = a.sink ? a.sink[head] * kLog2e : -INFINITY;
+  if (l < kWeightless) return l > 0.f && s == -INFINITY ? NAN : 0.f;
+  return 1.f / (l + __builtin_amdgcn_exp2f(s - m));
+}
 
 __device__ __forceinline__ float lane4_max(float x) {  // over the four lanes of a column
   const auto r16 = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -267,7 +281,7 @@ __device__ __forceinline__ void rows_body(const AttnArgs& a, uint8_t* lds, uint3
     for (int g = 0; g < DG; ++g)
 #pragma unroll
       for (int i = 0; i < 2; ++i) qf[g][i] = *reinterpret_cast<const bf16x8_t*>(qrow + 64 * g + 16 * q + 8 * i);
-    float m = -INFINITY, l = 0.f;
+    float m = kLowest, l = 0.f;
     f32x4_t o[DT];
 #pragma unroll
     for (int j = 0; j < DT; ++j) o[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
@@ -319,12 +333,11 @@ __device__ __forceinline__ void rows_body(const AttnArgs& a, uint8_t* lds, uint3
           bm = fmaxf(bm, v);
         }
       bm = lane4_max(bm);
-      const float mn = fmaxf(m, bm);
-      const float ref = mn == -INFINITY ? 0.f : mn;
+      const float ref = fmaxf(m, bm);
       const float alpha = __builtin_amdgcn_exp2f(m - ref);
-      m = mn;
+      m = ref;
       bf16x8_t p[2];
-      float sum = 0.f;
+      float sum = !edge || min(hi, t0 + kBlock) > max(row_lo, t0) ? kSeen : 0.f;
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
         float e[4];
@@ -392,13 +405,12 @@ __device__ __forceinline__ void rows_body(const AttnArgs& a, uint8_t* lds, uint3
       sl[wave][c] = l;
     }
     __syncthreads();
-    float M = -INFINITY, L = 0.f;
+    float M = kLowest, L = 0.f;
 #pragma unroll
     for (int w = 0; w < NW; ++w) M = fmaxf(M, sm[w][c]);
-    const float ref = M == -INFINITY ? 0.f : M;
 #pragma unroll
-    for (int w = 0; w < NW; ++w) L += sl[w][c] * __builtin_amdgcn_exp2f(sm[w][c] - ref);
-    const float f = __builtin_amdgcn_exp2f(m - ref);
+    for (int w = 0; w < NW; ++w) L += sl[w][c] * __builtin_amdgcn_exp2f(sm[w][c] - M);
+    const float f = __builtin_amdgcn_exp2f(m - M);
 #pragma unroll
     for (int j = 0; j < DT; ++j) o[j] *= f;
     if (wave >= NW / 2)
@@ -422,14 +434,8 @@ __device__ __forceinline__ void rows_body(const AttnArgs& a, uint8_t* lds, uint3
       t[4] = slot + 1;
       t[5] = 2;
     }
-    float inv = 0.f;
-    if (whole) {
-      // thread -> (4 dims, row c): c stays tid's
-      const float s_ = a.sink ? a.sink[head] * kLog2e : -INFINITY;
-      // a row without keys is zero, whatever its sink
-      const float den = L + __builtin_amdgcn_exp2f(s_ - ref);
-      inv = M == -INFINITY ? L : 1.f / den;  // L is 0 there, or not a number where every score is not
-    }
+    // thread -> (4 dims, row c): c stays tid's
+    const float inv = whole ? row_factor(a, head, M, L) : 0.f;
     for (int i = tid; i < DT * 4 * 16; i += 64 * NW) {
       f32x4_t v = so[0][i];
 #pragma unroll
@@ -476,8 +482,7 @@ __global__ void __launch_bounds__(256) paged_attn_join_kernel(const AttnArgs a, 
   const int step = t[5];
   auto finish = [&](int row, float m, float l, f32x4_t o) {
     const int head = h * a.group + row % a.group;
-    const float s_ = a.sink ? a.sink[head] * kLog2e : -INFINITY;
-    const float inv = m == -INFINITY ? l : 1.f / (l + __builtin_amdgcn_exp2f(s_ - m));
+    const float inv = row_factor(a, head, m, l);
     uint2 pk;
     pk.x = (uint32_t)f32_bf16(o[0] * inv) | ((uint32_t)f32_bf16(o[1] * inv) << 16);
     pk.y = (uint32_t)f32_bf16(o[2] * inv) | ((uint32_t)f32_bf16(o[3] * inv) << 16);
@@ -487,16 +492,15 @@ __global__ void __launch_bounds__(256) paged_attn_join_kernel(const AttnArgs a, 
     for (int i = blockIdx.z * SG + g; i < t[1]; i += gridDim.z * SG) {
       const int64_t first = t[3] + i / 16, second = t[4] + i / 16;
       const int c = i % 16;
-      float m = -INFINITY;
+      float m = kLowest;
 #pragma unroll 4
       for (int p = 0; p < n; ++p) m = fmaxf(m, a.part_ml[(p ? second + (int64_t)step * (p - 1) : first) * 32 + c]);
-      const float ref = m == -INFINITY ? 0.f : m;
       f32x4_t o = {0.f, 0.f, 0.f, 0.f};
       float l = 0.f;
 #pragma unroll 4
       for (int p = 0; p < n; ++p) {
         const int64_t slot = p ? second + (int64_t)step * (p - 1) : first;
-        const float f = __builtin_amdgcn_exp2f(a.part_ml[slot * 32 + c] - ref);
+        const float f = __builtin_amdgcn_exp2f(a.part_ml[slot * 32 + c] - m);
         l += f * a.part_ml[slot * 32 + 16 + c];
         o += *reinterpret_cast<const f32x4_t*>(a.part_o + (slot * 16 + c) * D + 4 * d) * f;
       }
@@ -507,19 +511,18 @@ __global__ void __launch_bounds__(256) paged_attn_join_kernel(const AttnArgs a, 
   for (int i = blockIdx.z; i < t[1]; i += gridDim.z) {
     const int64_t first = t[3] + i / 16, second = t[4] + i / 16;
     const int c = i % 16;
-    float m = -INFINITY;
+    float m = kLowest;
     for (int p = tid; p < n; p += 256) m = fmaxf(m, a.part_ml[(p ? second + (int64_t)step * (p - 1) : first) * 32 + c]);
     m = wave_max_f32(m);
     if ((tid & 63) == 0) red[tid >> 6] = m;
     __syncthreads();
     m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-    const float ref = m == -INFINITY ? 0.f : m;
     f32x4_t o = {0.f, 0.f, 0.f, 0.f};
     float l = 0.f;
 #pragma unroll 8
     for (int p = g; p < n; p += SG) {
       const int64_t slot = p ? second + (int64_t)step * (p - 1) : first;
-      const float f = __builtin_amdgcn_exp2f(a.part_ml[slot * 32 + c] - ref);
+      const float f = __builtin_amdgcn_exp2f(a.part_ml[slot * 32 + c] - m);
       l += f * a.part_ml[slot * 32 + 16 + c];
       o += *reinterpret_cast<const f32x4_t*>(a.part_o + (slot * 16 + c) * D + 4 * d) * f;
     }
@@ -691,7 +694,7 @@ __device__ __forceinline__ void tile_body(const AttnArgs& a, uint8_t* buf, int g
     return a.codes + wave * CPW * 1024 + at;
   };
 
-  float ref = -INFINITY, l = 0.f;  // ref: what a row's exponents are taken against
+  float ref = kLowest, l = 0.f;  // ref: what a row's exponents are taken against
   f32x16_t o[DQ];
   const f32x16_t zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -753,12 +756,13 @@ __device__ __forceinline__ void tile_body(const AttnArgs& a, uint8_t* buf, int g
     for (int i = 1; i < 16; ++i) bm = fmaxf(fmaxf(bm, s[0][i]), s[1][i]);
     return half_max(bm);
   };
-  // The reference of every row moves to its maximum with these scores.  A row
-  // without one (-inf) makes its next exponential infinite, which calls for this.
+  // The reference of every row moves to its maximum with these scores.  A row that has
+  // none yet (fp32's lowest number) makes its next exponential infinite, which calls for
+  // this; one of a score of -inf is 0, and does not.
   auto move = [&]() __attribute__((always_inline)) {
     const float top = largest() * a.scale;
     const bool go = top > ref;
-    const float alpha = go && ref != -INFINITY ? __builtin_amdgcn_exp2f(ref - top) : 1.f;
+    const float alpha = go ? __builtin_amdgcn_exp2f(ref - top) : 1.f;
     ref = go ? top : ref;
     l *= alpha;
 #pragma unroll
@@ -767,13 +771,13 @@ __device__ __forceinline__ void tile_body(const AttnArgs& a, uint8_t* buf, int g
   bf16x8_t p[4];
   // -> the lane's largest; their sum is added to l by the caller
   float sum;
-  auto exponentials = [&](auto fused, float to) __attribute__((always_inline)) -> float {
+  auto exponentials = [&](auto fused, float to, float seen) __attribute__((always_inline)) -> float {
     // one rounding, or two: with those, the maximum's exponent is 0 however large the scores are
     auto power = [&](float x) __attribute__((always_inline)) {
       return __builtin_amdgcn_exp2f(decltype(fused)::value ? __builtin_fmaf(x, a.scale, -to) : x * a.scale - to);
     };
     float big = 0.f;
-    sum = 0.f;
+    sum = seen;
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -806,7 +810,7 @@ __device__ __forceinline__ void tile_body(const AttnArgs& a, uint8_t* buf, int g
     load_values(kb);
     load_keys(next, 0, k0);
     __builtin_amdgcn_sched_barrier(0);
-    if (__ballot(exponentials(std::true_type{}, ref) > kLazy)) return false;
+    if (__ballot(exponentials(std::true_type{}, ref, kSeen) > kLazy)) return false;
     l += sum;
     __builtin_amdgcn_sched_barrier(0);
     products(e8m0_f32(ve));
@@ -826,7 +830,7 @@ __device__ __forceinline__ void tile_body(const AttnArgs& a, uint8_t* buf, int g
         s[t][i] = at < see_hi && at >= see_lo ? (ke == 255u ? NAN : s[t][i]) : -INFINITY;
       }
     move();
-    exponentials(std::false_type{}, ref == -INFINITY ? 0.f : ref);
+    exponentials(std::false_type{}, ref, min(good ? row_hi : 0, t0 + kBlock) > max(row_lo, t0) ? kSeen : 0.f);
     l += sum;
     __builtin_amdgcn_sched_barrier(0);
     load_values(kb);
@@ -933,9 +937,8 @@ __device__ __forceinline__ void tile_body(const AttnArgs& a, uint8_t* buf, int g
   }
   l = half_sum(l);
   if (gridDim.y == 1) {
-    const float s_ = a.sink ? a.sink[head] * kLog2e : -INFINITY;
-    const float inv = ref == -INFINITY ? l : 1.f / (l + __builtin_amdgcn_exp2f(s_ - ref));
     if (own_row) {
+      const float inv = row_factor(a, head, ref, l);
       uint16_t* orow = a.out + ((int64_t)(x.s0 + tok) * a.hq + head) * D;
 #pragma unroll
       for (int j = 0; j < DQ; ++j)

@@ -1191,7 +1191,8 @@ def paged_attention(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, 
     seq_lens[r] - (its rows) + t and sees the tokens up to itself, with ``window``
     only that many of them; ``sink`` [Hq] f32 adds exp(sink) to the denominator.
     Decode steps, drafts, pieces of prompts and whole prompts may share a call.
-    Rows without a key and rows behind the last request are zero.  ``max_new``:
+    Rows without a key and rows behind the last request are zero; a row whose
+    scores are all -inf is not a number, or zero beside a sink.  ``max_new``:
     the most rows of any request where the caller knows it (it only sizes the
     launches).  ``starts`` ascends from 0.  ``out`` may not overlap q.  Requests may
     share pages (a common prefix).  A ``workspace`` serves one call at a time: calls on other

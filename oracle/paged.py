@@ -175,8 +175,10 @@ def attention(q, codes, scales, table, starts, seq, scale, sink=None, window=0):
                 kk, vv = k[h // (hq // hkv), see], v[h // (hq // hkv), see]
                 s = kk @ q[j, h] * scale
                 m = s.max() if not np.isnan(s).any() else np.nan
-                p = np.exp(s - m)
-                den = p.sum() + (math.exp(sink[h] - m) if sink is not None else 0.0)
+                low = m == -np.inf  # every score: weights of 0, which leave the sink, or 0 / 0
+                p = np.zeros_like(s) if low else np.exp(s - m)
+                den = p.sum() + (math.exp(sink[h] - (0.0 if low else m)) if sink is not None else 0.0)
+                den = den if den else np.nan
                 o[j, h] = p @ vv / den
                 ds = float(np.max((d + 2) * u * abs(scale) * (np.abs(kk) @ np.abs(q[j, h])) + 4 * u * np.abs(s)))
                 a = p @ np.abs(vv) / den

@@ -643,3 +643,59 @@ def test_refusals_of_the_wrappers(dev):
                dict(out=ops.PagedStep.empty(2, 3, dev)), dict(lengths=same, out=ops.PagedStep(z(3), same, z(1), z(2), z(2), z(2)))):
         with pytest.raises((ValueError, TypeError)):
             ops.paged_step(**{**ok, **kw})
+
+
+# --------------------------------------------------- the ends of the range ----
+def _attend(dev, q, c, s, table, starts, seq, scale, sink=None, window=0):
+    from mosaic_amd import ops
+    q = torch.from_numpy(np.asarray(q, np.float32)).to(dev).to(torch.bfloat16)
+    snk = None if sink is None else torch.from_numpy(sink).to(dev)
+    return ops.paged_attention(q, torch.from_numpy(c).to(dev), torch.from_numpy(s).to(dev), _i32(table, dev),
+                               _i32(starts, dev), _i32(seq, dev), scale, sink=snk,
+                               window=window).float().cpu().numpy().astype(np.float64)
+
+
+# rows of a request that the few-row kernel finishes itself, cuts and joins, and the same of many rows
+KINDS = [([150, 130], [3, 1]), ([3000, 140], [1, 2]), ([140], [40]), ([3000], [40])]
+
+
+@pytest.mark.parametrize("sink", [False, True])
+@pytest.mark.parametrize("held,new", KINDS)
+def test_attention_scores_below_the_range(dev, held, new, sink):
+    """Keys whose scores overflow to -inf weigh nothing beside later ones, however many blocks they fill."""
+    rng = np.random.default_rng(40)
+    table, total, starts, seq = _batch(rng, held, new, 64)
+    c, s = _cache(rng, total, 1, 2, 64)
+    c[:, :, :, 0] = 0  # scores of 0
+    for i in range(len(held)):
+        for b in table[i, :2]:  # the first 128 tokens: every dim at least 2^-6 2^60 below 0, times 2^100 and more
+            c[b, :, :, 0] = 0x80 | rng.integers(8, 0x7F, c[b, :, :, 0].shape).astype(np.uint8)
+            s[b, :, :, 0] = 127 + 60
+    t = int(starts[-1])
+    q = np.exp2(rng.integers(100, 110, (t, 4, 64)).astype(np.float64))
+    snk = rng.standard_normal(4).astype(np.float32) if sink else None
+    o = _attend(dev, q, c, s, table, starts, seq, 0.125, snk)
+    # the same without these keys, and without what no longer matters, the size of the queries
+    hidden = table.copy()
+    hidden[:, :2] = -1
+    want, tol = P.attention(np.zeros_like(q), c, s, hidden, starts, seq, 0.125, snk)
+    assert np.isfinite(o).all() and np.all(np.abs(o - want) <= tol)
+
+
+@pytest.mark.parametrize("held,new", KINDS)
+def test_attention_rows_of_scores_all_minus_infinity(dev, held, new):
+    """0 / 0 where there is no sink, and 0 beside one; rows that see no key are 0 in either case."""
+    rng = np.random.default_rng(41)
+    table, total, starts, seq = _batch(rng, held + [0, 0], new + [2, 20], 64)
+    c, s = _cache(rng, total, 1, 2, 64)
+    at_k = P.block_maps(64)[0]
+    c[:, :, :, 0, at_k[:, 5]] = 0x80 | rng.integers(1, 0x7F, (total, 1, 2, 64)).astype(np.uint8)  # below 0
+    table[-2:] = -1  # requests without pages
+    q = _bf16(rng, int(starts[-1]), 4, 64).astype(np.float64)
+    q[..., 5] = np.inf
+    keyless = np.arange(int(starts[-1])) >= starts[-3]
+    plain = _attend(dev, q, c, s, table, starts, seq, 0.125)
+    assert np.isnan(plain[~keyless]).all() and not plain[keyless].any()
+    assert not _attend(dev, q, c, s, table, starts, seq, 0.125, np.zeros(4, np.float32)).any()
+    want, _ = P.attention(q, c, s, table, starts, seq, 0.125)
+    np.testing.assert_array_equal(np.isnan(plain), np.isnan(want))
