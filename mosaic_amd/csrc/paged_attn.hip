@@ -1167,8 +1167,9 @@ extern "C" int mosaic_paged_attention(const uint16_t* q, int64_t q_token_stride,
   a.pages = (int)pages;
   a.nb = (int)blocks;
   a.window = window >= (1 << 30) ? 0 : (int)window;  // longer than any context: none
-  // a scale of zero is one too small to move a score (the masked ones stay at -inf)
-  a.scale = fmaxf(fabsf(softmax_scale) * kLog2e, 1e-37f);
+  // Finite and not zero, or a score of 0, or a masked one, would be no number: a scale of zero is fp32's
+  // least number, which brings no product of fp32's range to more than 2^-21.
+  a.scale = fminf(fmaxf(fabsf(softmax_scale) * kLog2e, 0x1p-149f), -kLowest);
   a.sign = softmax_scale < 0.f ? -1.f : 1.f;
   const int64_t rows = (max_new && max_new < tokens ? max_new : tokens) * a.group;
   const int few_rows = (int)(rows < kRows ? rows : kRows);

@@ -699,3 +699,22 @@ def test_attention_rows_of_scores_all_minus_infinity(dev, held, new):
     assert not _attend(dev, q, c, s, table, starts, seq, 0.125, np.zeros(4, np.float32)).any()
     want, _ = P.attention(q, c, s, table, starts, seq, 0.125)
     np.testing.assert_array_equal(np.isnan(plain), np.isnan(want))
+
+
+@pytest.mark.parametrize("scale", [0.0, 2.0 ** -130, 3e38, -3e38])
+@pytest.mark.parametrize("held,new", KINDS)
+def test_attention_scales_at_the_ends(dev, held, new, scale):
+    """A scale of 0, or one that brings large scores back to where they do not count, gives means; so does the
+    largest where every score is 0."""
+    rng = np.random.default_rng(42)
+    table, total, starts, seq = _batch(rng, held, new, 64)
+    c, s = _cache(rng, total, 1, 2, 64)
+    q = _bf16(rng, int(starts[-1]), 4, 64).astype(np.float64) * (2.0 ** 116 if abs(scale) < 1 else 0.0)
+    want, tol = P.attention(q, c, s, table, starts, seq, scale)
+    if abs(scale) < 1:  # the products are within fp32's range
+        for i in range(len(held)):
+            k = P.gather(c, s, table[i], int(seq[i]))[0]
+            rows = q[starts[i]:starts[i + 1]]
+            assert max(float((np.abs(k[h // 2]) @ np.abs(rows[:, h]).T).max()) for h in range(4)) < 2.0 ** 128
+    o = _attend(dev, q, c, s, table, starts, seq, scale)
+    assert np.all(np.abs(o - want) <= tol)
