@@ -571,7 +571,8 @@ int mosaic_paged_trim(const int32_t* lengths, const int32_t* keep, const int32_t
  * (strides in elements, multiples of 8; 16-byte aligned; head_dim 64, 128 or
  * 256) into the cache.  A block and head's scale is the least power of two 2^e,
  * e >= -126, with its largest finite magnitude at most 448 2^e; codes are
- * e4m3(x / 2^e), nearest even, infinities to +-448, NaN kept.  Where a block
+ * e4m3(x / 2^e), nearest even, infinities to +-448, NaN kept; where e = 120 codes
+ * are at most 240, since 256 2^120 is no number of bf16.  Where a block
  * held tokens before, its scale only grows, and the old codes are rounded to
  * the new one; the rest of a block that begins in this call is zeroed, bytes
  * behind the last token of an older one are left.  Blocks that take new tokens

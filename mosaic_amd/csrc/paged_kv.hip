@@ -240,12 +240,14 @@ __device__ __forceinline__ int scale_exp(uint32_t amax_bits) {
 __device__ __forceinline__ float pow2f(int e) {  // -126 <= e <= 127
   return __uint_as_float((uint32_t)(e + 127) << 23);
 }
-// four values as e4m3 bytes, nearest even.  ODD: infinities go to +-448 and NaN stays
-// NaN; without it |x| is at most 448.
+// The largest code that is finite times 2^e: 448, and 240 for e = 120 (1.875 2^127; 256 would be 2^128)
+__device__ __forceinline__ float largest_code(int e) { return fminf(1.875f * pow2f(127 - max(e, 1)), 448.f); }
+// four values as e4m3 bytes, nearest even.  ODD: what is larger goes to +-top, infinities
+// too, and NaN stays NaN; without it |x| is at most 448, and top too.
 template <bool ODD>
-__device__ __forceinline__ uint32_t to_e4m3(float a, float b, float c, float d) {
+__device__ __forceinline__ uint32_t to_e4m3(float a, float b, float c, float d, float top) {
   if constexpr (ODD) {
-    auto fit = [](float x) { return x == x ? fminf(fmaxf(x, -448.f), 448.f) : x; };
+    auto fit = [=](float x) { return x == x ? fminf(fmaxf(x, -top), top) : x; };
     a = fit(a);
     b = fit(b);
     c = fit(c);
@@ -372,7 +374,7 @@ __global__ void __launch_bounds__(256) paged_kv_write_kernel(const WriteArgs a) 
 #pragma unroll
     for (int part = 0; part < 2; ++part) {
       // 2^-e by halves: e = 128 (a NaN scale that was written by someone else) has no normal inverse
-      const float i0 = pow2f(-(e[part] / 2)), i1 = pow2f(-(e[part] - e[part] / 2));
+      const float i0 = pow2f(-(e[part] / 2)), i1 = pow2f(-(e[part] - e[part] / 2)), top = largest_code(e[part]);
 #pragma unroll
       for (int i = 0; i < G; ++i)
 #pragma unroll
@@ -380,11 +382,11 @@ __global__ void __launch_bounds__(256) paged_kv_write_kernel(const WriteArgs a) 
           const uint32_t w0 = x[part][i][j >> 1][2 * (j & 1)], w1 = x[part][i][j >> 1][2 * (j & 1) + 1];
           code[part][i][j] = to_e4m3<decltype(odd_)::value>(
               __uint_as_float(w0 << 16) * i0 * i1, __uint_as_float(w0 & 0xFFFF0000u) * i0 * i1,
-              __uint_as_float(w1 << 16) * i0 * i1, __uint_as_float(w1 & 0xFFFF0000u) * i0 * i1);
+              __uint_as_float(w1 << 16) * i0 * i1, __uint_as_float(w1 & 0xFFFF0000u) * i0 * i1, top);
         }
     }
   };
-  if (odd)
+  if (odd || max(e[0], e[1]) >= 120)
     encode(std::true_type{});
   else
     encode(std::false_type{});

@@ -1163,9 +1163,10 @@ def paged_kv_write(k: torch.Tensor, v: torch.Tensor, codes: torch.Tensor, scales
     """Write a step's keys and values k, v [T, Hkv, D] bf16 (D = 64, 128 or 256)
     into the paged cache, 8 bits a value: ``codes`` [P, NB, Hkv, 2, 64 D] e4m3 and
     ``scales`` [P, NB, Hkv, 2] e8m0, one scale a block of 64 tokens and head,
-    2^e with the largest magnitude at most 448 2^e.  ``starts`` (ascending from 0) and ``seq_lens`` as in
-    ``PagedStep``; no block that takes new tokens may be in two requests' tables.  A block that held tokens before keeps its scale or moves to a
-    larger one; the rest of a block that begins here is zeroed."""
+    2^e with the largest finite magnitude at most 448 2^e (at e = 120, where 256 2^e is infinite,
+    codes end at 240).  ``starts`` (ascending from 0) and ``seq_lens`` as in ``PagedStep``; no block
+    that takes new tokens may be in two requests' tables.  A block that held tokens before keeps its
+    scale or moves to a larger one; the rest of a block that begins here is zeroed."""
     (k, k_at, k_tok, k_head), (v, v_at, v_tok, v_head) = _paged_rows(k, "k"), _paged_rows(v, "v")
     dev = k.get_device()
     if v.get_device() != dev or v.shape != k.shape:

@@ -86,6 +86,11 @@ def scale_exp(amax: float) -> int:
     return max(e, -126)
 
 
+def largest_code(e: int) -> float:
+    """The largest e4m3 value that is below 2^128 times 2^e."""
+    return min(448.0, 1.875 * 2.0 ** (127 - e))
+
+
 def write(k, v, codes, scales, table, starts, seq):
     """k, v [T, Hkv, D] float64 -> codes [P, NB, Hkv, 2, 64 D] and scales [P, NB, Hkv, 2] updated in place."""
     nb, hkv, d = codes.shape[1], codes.shape[2], codes.shape[4] // BLOCK
@@ -115,7 +120,8 @@ def write(k, v, codes, scales, table, starts, seq):
                         e = max(e, was)
                     else:
                         unit[at[hi:]] = 0
-                    y = np.where(np.isnan(new), new, np.clip(new * 2.0 ** -e, -448.0, 448.0))
+                    top = largest_code(e)
+                    y = np.where(np.isnan(new), new, np.clip(new * 2.0 ** -e, -top, top))
                     unit[at[lo:hi]] = C.e4m3_encode(y.astype(np.float32))
                     scales[page, sub, h, part] = e + 127
 

@@ -718,3 +718,30 @@ def test_attention_scales_at_the_ends(dev, held, new, scale):
             assert max(float((np.abs(k[h // 2]) @ np.abs(rows[:, h]).T).max()) for h in range(4)) < 2.0 ** 128
     o = _attend(dev, q, c, s, table, starts, seq, scale)
     assert np.all(np.abs(o - want) <= tol)
+
+
+@pytest.mark.parametrize("n", [3, 40])
+def test_values_near_the_largest_are_read_back(dev, n):
+    """bf16's largest values, and infinities among them, are written so that what is read back is a number."""
+    from mosaic_amd import ops
+    rng = np.random.default_rng(43)
+    hkv, d, t = 2, 64, n
+    codes, scales = _cache(rng, 2, 1, hkv, d)
+    x = np.exp2(127.0) * (1 + rng.integers(0, 128, (t, hkv, d)) / 128) * np.where(rng.random((t, hkv, d)) < 0.5, -1, 1)
+    x[0] = 2.0 ** 127 * (2 - 2.0 ** -7)
+    bad = rng.random((t, hkv, d)) < 0.1
+    bad[0] = False
+    xt = torch.from_numpy(np.where(bad, np.sign(x) * np.inf, x).astype(np.float32)).to(dev).to(torch.bfloat16)
+    ct, st = torch.from_numpy(codes).to(dev), torch.from_numpy(scales).to(dev)
+    table, starts, seq = _i32([[1]], dev), _i32([0, t], dev), _i32([t], dev)
+    ops.paged_kv_write(xt, xt, ct, st, table, starts, seq)
+    P.write(xt.double().cpu().numpy(), xt.double().cpu().numpy(), codes, scales, table.cpu().numpy(), [0, t], [t])
+    np.testing.assert_array_equal(st.cpu().numpy(), scales)
+    _same_codes(ct.cpu().numpy(), codes)
+    # one key a row: the value itself
+    q = torch.zeros(t, hkv, d, dtype=torch.bfloat16, device=dev)
+    o = ops.paged_attention(q, ct, st, table, starts, seq, 0.125, window=1).float().cpu().numpy().astype(np.float64)
+    assert np.isfinite(o).all()
+    # at most 2^-4 off, half a step of e4m3; the codes above 240 are not used, 15/255 of the largest
+    assert np.all(np.abs(o - x)[~bad] <= 2.0 ** -4 * np.abs(x)[~bad])
+    np.testing.assert_array_equal(o[bad], np.sign(x)[bad] * 240.0 * 2.0 ** 120)
