@@ -526,7 +526,9 @@ int mosaic_dsa_decode_indices(const int32_t* pos, int64_t rows, int64_t window, 
 /* ----------------------------------------------------- paged KV cache ---- */
 /* One pool of pages holds the keys and values of many requests in 8 bits:
  * codes [pages, blocks, kv_heads, 2, 64 head_dim] e4m3 and scales [pages,
- * blocks, kv_heads, 2] e8m0 (the value is code * 2^(scale - 127)).  A page is
+ * blocks, kv_heads, 2] e8m0: the value is code * 2^(scale - 127), read as bf16 (below
+ * 2^-126 in its steps of 2^-133), and 255 is not a number.  Magnitudes of 2^128 and more,
+ * which the writer does not make, are infinite as keys and not numbers as values.  A page is
  * `blocks` (1..64) blocks of 64 tokens, page_size = 64 blocks; index 0 of the
  * last but one axis holds keys, 1 values.  The bytes of a block are
  *   keys   [4 tg][head_dim/64 dg][4 q][16 c][16 j]: token 16 tg + c, dim 64 dg + 16 q + j
@@ -591,6 +593,8 @@ int mosaic_paged_kv_write(const uint16_t* k, const uint16_t* v, int64_t k_token_
  * exp(sink) to the softmax denominator.  out [tokens, q_heads, head_dim] bf16,
  * contiguous; rows without a key, and rows behind the last request, are zero, and
  * rows whose keys' scores are all -inf are 0 / 0 without a sink and 0 with one.
+ * Weights times values are summed in fp32 before the division: beside values near
+ * 2^127 a row's sum may pass its range where its mean would not.
  * max_new: the most rows of any request, or 0 if not known (it only sizes the
  * launch).  starts ascends from 0 and out may not overlap q.  The workspace may be
  * NULL where the query says 0 bytes. */

@@ -2,7 +2,8 @@
 // a ragged batch sees its request's tokens up to its own position, optionally
 // only the last `window` of them, with an optional sink logit for each head.
 //
-//   s = scale q . k in fp32 (k = code 2^(e - 127), exact in bf16), running
+//   s = scale q . k in fp32 (k = code 2^(e - 127) in bf16: exact from 2^-126 on,
+//   rounded to its step of 2^-133 below, infinite from 2^128 on), running
 //   maximum and sum of exp(s - m) in fp32, o = sum p v / (sum p + exp(sink - m)).
 //   p is rounded to bf16 for the matrix unit's value product: at most 2^-8 of a
 //   term, of either sign, as much as the bf16 output's own rounding.  Sums are
@@ -128,7 +129,8 @@ __device__ __forceinline__ float lane4_sum(float x) {
   return __uint_as_float(r32[0]) + __uint_as_float(r32[1]);
 }
 
-// eight codes (two words) times 2^n, exact in bf16
+// Eight codes (two words) times a scale byte's 2^(e - 127) in bf16, by the exponent of
+// `scale`: 2^-127 for byte 0, though that is 0 as a float.
 __device__ __forceinline__ bf16x8_t to_bf16(uint32_t w0, uint32_t w1, float scale) {
   const bf16x2_t a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w0, scale, false);
   const bf16x2_t b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w0, scale, true);
@@ -137,11 +139,19 @@ __device__ __forceinline__ bf16x8_t to_bf16(uint32_t w0, uint32_t w1, float scal
   return bf16x8_t{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
-// 0xFF in every byte of w that is a NaN code (0x7F or 0xFF)
-__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {
-  const uint32_t x = ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;  // the high bit of a byte: it was 0x7F
+// The least code that is no finite number at scale byte e: NaN's, 0x7F; from byte 247 on the
+// one of 2^(255 - e), which times 2^(e - 127) is 2^128 (zero times that is no number either); at
+// 255 any.  As what is to be added to a byte's magnitude for its high bit, in every byte.
+constexpr uint32_t kOverflow = 247;  // the least scale byte at which codes pass the range
+__device__ __forceinline__ uint32_t bad_from(uint32_t e) {
+  return (e < kOverflow ? 1u : e == 255u ? 0x80u : 0x80u - 8u * (262u - e)) * 0x01010101u;
+}
+// 0xFF in every byte of w that is such a code
+__device__ __forceinline__ uint32_t bad_bytes(uint32_t w, uint32_t from) {
+  const uint32_t x = ((w & 0x7F7F7F7Fu) + from) & 0x80808080u;
   return x | (x - (x >> 7));
 }
+constexpr uint32_t kNan = 0x01010101u;  // bad_from of the ordinary scales
 
 // The units of all requests are numbered through, `units(request)` of each, and so
 // are their row tiles, `tiles(request)`.  Finds the request that holds unit
@@ -315,8 +325,8 @@ __device__ __forceinline__ void rows_body(const AttnArgs& a, uint8_t* lds, uint3
             s[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(to_bf16(kw[t][g][2 * i], kw[t][g][2 * i + 1], ks), qf[g][i],
                                                            s[t], 0, 0, 0);
       }
-      // a block that some row does not see whole, one without a page, or of a NaN scale
-      const bool edge = t0 + kBlock > all_hi || t0 < all_lo || !good || ke == 255u || ve == 255u;
+      // a block that some row does not see whole, one without a page, or whose scale makes no numbers
+      const bool edge = t0 + kBlock > all_hi || t0 < all_lo || !good || ke == 255u || ve >= kOverflow;
       const int hi = good ? row_hi : 0;
       float bm = -INFINITY;
 #pragma unroll
@@ -357,15 +367,20 @@ __device__ __forceinline__ void rows_body(const AttnArgs& a, uint8_t* lds, uint3
 #pragma unroll
       for (int j = 0; j < DT; ++j) o[j] *= alpha;
       if (edge) {
-        // A code that is not a number reaches only the rows that see its token: it is
-        // taken out of the product (zero times it would reach all), and where a
+        // A code that is not a finite number reaches only the rows that see its token: it
+        // is taken out of the product (zero times it would reach all), and where a
         // count of the seen ones is not zero, the result is not a number.
+        if (ve >= kOverflow)  // seldom: NaN codes for all of them
+#pragma unroll
+          for (int j = 0; j < DT; ++j)
+#pragma unroll
+            for (int w = 0; w < 4; ++w) vw[j][w] |= bad_bytes(vw[j][w], bad_from(ve));
         uint32_t any = 0u;
 #pragma unroll
         for (int j = 0; j < DT; ++j)
 #pragma unroll
-          for (int w = 0; w < 4; ++w) any |= nan_bytes(vw[j][w]);
-        if (__ballot(any != 0u || ve == 255u)) {
+          for (int w = 0; w < 4; ++w) any |= bad_bytes(vw[j][w], kNan);
+        if (__ballot(any != 0u)) {
           bf16x8_t see[2];
 #pragma unroll
           for (int t = 0; t < 4; ++t)
@@ -379,7 +394,7 @@ __device__ __forceinline__ void rows_body(const AttnArgs& a, uint8_t* lds, uint3
             uint32_t bad[4];
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
-              bad[w] = ve == 255u ? 0xFFFFFFFFu : nan_bytes(vw[j][w]);
+              bad[w] = bad_bytes(vw[j][w], kNan);
               vw[j][w] &= ~bad[w];
               bad[w] &= 0x38383838u;  // the code of 1
             }
@@ -816,7 +831,7 @@ __device__ __forceinline__ void tile_body(const AttnArgs& a, uint8_t* buf, int g
     products(e8m0_f32(ve));
     return true;
   };
-  // any other: one that some row does not see whole, without a page, or of a scale that is no number
+  // any other: one that some row does not see whole, without a page, or whose scale makes no numbers
   auto edge_block = [&](const uint8_t* kb, int t0, bool good, uint32_t ke, uint32_t ve) __attribute__((always_inline)) {
     load_keys(kb, 0, k0);
     scores(std::false_type{}, kb, e8m0_f32(ke));
@@ -834,15 +849,16 @@ __device__ __forceinline__ void tile_body(const AttnArgs& a, uint8_t* buf, int g
     l += sum;
     __builtin_amdgcn_sched_barrier(0);
     load_values(kb);
-    // A code that is not a number reaches only the rows that see its token (see the
-    // kernel above): it is taken out, and where a count of the seen ones is not zero,
-    // the result is not a number.
+    // A code that is not a finite number reaches only the rows that see its token (see
+    // the kernel above): it is taken out, and where a count of the seen ones is not
+    // zero, the result is not a number.
+    const uint32_t from = bad_from(ve);
     uint32_t any = 0u;
 #pragma unroll
     for (int j = 0; j < DQ; ++j)
 #pragma unroll
-      for (int w = 0; w < 8; ++w) any |= (vw[j][w >> 2][w & 3] & 0x7F7F7F7Fu) + 0x01010101u;
-    if (__ballot((any & 0x80808080u) != 0u || ve == 255u)) {
+      for (int w = 0; w < 8; ++w) any |= (vw[j][w >> 2][w & 3] & 0x7F7F7F7Fu) + from;
+    if (__ballot((any & 0x80808080u) != 0u)) {
       bf16x8_t see[4];
 #pragma unroll
       for (int w = 0; w < 4; ++w)
@@ -857,7 +873,7 @@ __device__ __forceinline__ void tile_body(const AttnArgs& a, uint8_t* buf, int g
         f32x16_t n = zero;
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-          const uint32_t ba = ve == 255u ? ~0u : nan_bytes(vw[j][0][w]), bb = ve == 255u ? ~0u : nan_bytes(vw[j][1][w]);
+          const uint32_t ba = bad_bytes(vw[j][0][w], from), bb = bad_bytes(vw[j][1][w], from);
           n = __builtin_amdgcn_mfma_f32_32x32x16_bf16(to_bf16(ba & 0x38383838u, bb & 0x38383838u, 1.f), see[w], n, 0, 0, 0);
         }
 #pragma unroll
@@ -868,7 +884,7 @@ __device__ __forceinline__ void tile_body(const AttnArgs& a, uint8_t* buf, int g
 #pragma unroll
       for (int j = 0; j < DQ; ++j)
 #pragma unroll
-        for (int w = 0; w < 8; ++w) vw[j][w >> 2][w & 3] &= ~(ve == 255u ? ~0u : nan_bytes(vw[j][w >> 2][w & 3]));
+        for (int w = 0; w < 8; ++w) vw[j][w >> 2][w & 3] &= ~bad_bytes(vw[j][w >> 2][w & 3], from);
     }
     products(ve == 255u ? 1.f : e8m0_f32(ve));
   };
@@ -912,7 +928,7 @@ __device__ __forceinline__ void tile_body(const AttnArgs& a, uint8_t* buf, int g
       bool edge = false;
       for (; b < nblk; leave()) {
         if (!again) arrive();
-        edge = t0 + kBlock > all_hi || t0 < all_lo || sc >= 0xFF00u || (sc & 0xFFu) == 255u;
+        edge = t0 + kBlock > all_hi || t0 < all_lo || sc >= kOverflow << 8 || (sc & 0xFFu) == 255u;
         if (edge) break;
         const bool done = whole_block(kb, next, sc & 0xFFu, sc >> 8);
         edge = !done && again;  // scores so large that a rounding of them is more than 8: two roundings

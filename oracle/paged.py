@@ -127,7 +127,8 @@ def write(k, v, codes, scales, table, starts, seq):
 
 
 def gather(codes, scales, table_row, length):
-    """The keys and values of one request, [Hkv, length, D] float64 each (scale byte 255: not a number)."""
+    """The keys and values of one request, [Hkv, length, D] float64 each (scale byte 255: not a number).
+    2^128 and more, which bf16 and fp32 do not have, are infinite keys and values that are not numbers."""
     nb, hkv, d = codes.shape[1], codes.shape[2], codes.shape[4] // BLOCK
     maps = block_maps(d)
     out = [np.full((hkv, -(-length // BLOCK) * BLOCK, d), np.nan) for _ in range(2)]
@@ -139,7 +140,9 @@ def gather(codes, scales, table_row, length):
             e = scales[page, b % nb, :, part].astype(np.int64) - 127
             s = np.where(e == 128, np.nan, np.exp2(e.astype(np.float64)))
             x = C.e4m3_decode(codes[page, b % nb, :, part]).astype(np.float64)[:, maps[part]]
-            out[part][:, BLOCK * b:BLOCK * (b + 1)] = x * s[:, None, None]
+            x = x * s[:, None, None]
+            past = np.abs(x) >= 2.0 ** 128
+            out[part][:, BLOCK * b:BLOCK * (b + 1)] = np.where(past, np.nan if part else np.copysign(np.inf, x), x)
     return out[0][:, :length], out[1][:, :length]
 
 
@@ -182,7 +185,7 @@ def attention(q, codes, scales, table, starts, seq, scale, sink=None, window=0):
                 s = kk @ q[j, h] * scale
                 m = s.max() if not np.isnan(s).any() else np.nan
                 low = m == -np.inf  # every score: weights of 0, which leave the sink, or 0 / 0
-                p = np.zeros_like(s) if low else np.exp(s - m)
+                p = np.zeros_like(s) if low else np.exp(s - m) if np.isfinite(m) else np.full_like(s, np.nan)
                 den = p.sum() + (math.exp(sink[h] - (0.0 if low else m)) if sink is not None else 0.0)
                 den = den if den else np.nan
                 o[j, h] = p @ vv / den

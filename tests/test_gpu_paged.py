@@ -745,3 +745,81 @@ def test_values_near_the_largest_are_read_back(dev, n):
     # at most 2^-4 off, half a step of e4m3; the codes above 240 are not used, 15/255 of the largest
     assert np.all(np.abs(o - x)[~bad] <= 2.0 ** -4 * np.abs(x)[~bad])
     np.testing.assert_array_equal(o[bad], np.sign(x)[bad] * 240.0 * 2.0 ** 120)
+
+
+@pytest.mark.parametrize("n", [2, 40])
+@pytest.mark.parametrize("byte", [0, 1, 2, 3, 100, 245, 246, 247, 248, 254])
+def test_values_of_every_code_and_scale(dev, n, byte):
+    """One key a row: the output is the code times 2^(byte - 127), rounded to bf16; 2^128 and more is not a
+    number, for the rows that see it alone."""
+    rng = np.random.default_rng(44)
+    c, s = _cache(rng, 5, 1, 1, 64)
+    all_codes = np.array([x for x in range(256) if x & 0x7F != 0x7F], np.uint8)
+    at_v = P.block_maps(64)[1]
+    held = 250 - n
+    for b in range(4):
+        c[b, 0, 0, 1, at_v] = np.resize(np.roll(all_codes, 37 * b), (64, 64))
+    s[..., 1] = byte
+    table = np.array([[0, 1, 2, 3]])
+    starts, seq = np.array([0, n]), np.array([held + n])
+    o = _attend(dev, np.zeros((n, 1, 64)), c, s, table, starts, seq, 0.125, window=1)
+    b = np.arange(held, held + n) // 64
+    v = C.e4m3_decode(c[table[0, b], 0, 0, 1]).astype(np.float64)[np.arange(n)[:, None], at_v[np.arange(held, held + n) % 64]]
+    v *= 2.0 ** (byte - 127)
+    fits = np.abs(v) < 2.0 ** 128
+    assert (byte < 247) == fits.all()
+    np.testing.assert_array_equal(np.isnan(o[:, 0]), ~fits)
+    off = np.abs(o[:, 0] - v)[fits]
+    # exact but below bf16's normal numbers, whose step is 2^-133
+    assert np.all(off <= np.where(np.abs(v[fits]) < 2.0 ** -126, 2.0 ** -134, 0.0)), off.max()
+
+
+@pytest.mark.parametrize("n", [2, 40])
+@pytest.mark.parametrize("byte", [0, 1, 6, 246, 254])
+def test_keys_of_the_ends_of_the_scales(dev, n, byte):
+    """Scores of keys at the ends of the range, brought to ordinary size by the queries."""
+    rng = np.random.default_rng(45)
+    table, total, starts, seq = _batch(rng, [100], [n], 64)
+    c, s = _cache(rng, total, 1, 2, 64)
+    s[..., 0] = byte
+    c[:, :, :, 0] = (c[:, :, :, 0] & 0xBF) | 0x20  # magnitudes of 2^-3 to 2^0.9: normal numbers in bf16 from byte 4 on
+    size = 2.0 ** (120 if byte < 127 else -118)
+    q = _bf16(rng, n, 4, 64).astype(np.float64) * size
+    scale = 2.0 ** (127 - byte) / size if byte < 127 else 2.0 ** -8
+    o = _attend(dev, q, c, s, table, starts, seq, scale)
+    want, tol = P.attention(q, c, s, table, starts, seq, scale)
+    assert np.all(np.abs(o - want) <= tol)
+
+
+@pytest.mark.parametrize("held,new", KINDS)
+@pytest.mark.parametrize("byte", [247, 250, 254])
+def test_attention_values_past_the_range_reach_only_rows_that_see_them(dev, held, new, byte):
+    """Values of 2^128 and more make the dim of every row that sees them no number, and of no other; keys of
+    that size have infinite scores, which weigh nothing below and leave no number above."""
+    rng = np.random.default_rng(46)
+    table, total, starts, seq = _batch(rng, held, new, 64)
+    c, s = _cache(rng, total, 1, 2, 64)
+    at_k, at_v = P.block_maps(64)
+    for i in range(len(held)):
+        last = int(seq[i]) - 1
+        for b, tok, dim, code in ((0, 3, 9, 0xFE), (last // 64, last % 64, 7, 0x7E)):  # all rows see it; one alone
+            s[table[i, b], 0, 1, 1] = byte
+            c[table[i, b], 0, 1, 1] = 0
+            c[table[i, b], 0, 1, 1, at_v[tok, dim]] = code
+        c[table[i, 1], 0, 0, 0] = 0
+        c[table[i, 1], 0, 0, 0, at_k[20]] = 0x7E
+        s[table[i, 1], 0, 0, 0] = byte
+    q = _bf16(rng, int(starts[-1]), 4, 64).astype(np.float64)
+    q[:, 0], q[:, 1] = np.abs(q[:, 0]) + 0.5, -np.abs(q[:, 1]) - 0.5
+    o = _attend(dev, q, c, s, table, starts, seq, 0.125)
+    assert np.isnan(o[:, 0]).all() and np.isfinite(o[:, 1]).all()
+    want, tol = P.attention(q, c, s, table, starts, seq, 0.125)
+    own = np.zeros(o[:, 2:].shape, bool)
+    own[..., 9] = True
+    own[starts[1:] - 1, :, 7] = True
+    np.testing.assert_array_equal(np.isnan(want[:, 2:]), own)
+    np.testing.assert_array_equal(np.isnan(o[:, 2:]), own)
+    assert np.all((np.abs(o - want) <= tol)[:, 2:][~own])
+    for i in range(len(held)):
+        s[table[i, 1], 0, 0, 0] = 240  # the same key, its score far below but finite
+    np.testing.assert_array_equal(_attend(dev, q, c, s, table, starts, seq, 0.125)[:, 1], o[:, 1])
