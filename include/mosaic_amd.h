@@ -552,7 +552,8 @@ int mosaic_dsa_decode_indices(const int32_t* pos, int64_t rows, int64_t window, 
  * where placed and 0 where not (the reader and writer below then skip the
  * request: its rows attend to nothing and give zeros); positions and slots
  * [tokens] (page id * page_size + offset; -1 for rows that are not placed or
- * behind the last request); *count_out: pages left.  Outputs may not overlap
+ * behind the last request, and slots of -1 where the table's id is below 0 or the
+ * slot not below 2^31); *count_out: pages left.  Outputs may not overlap
  * inputs (block_table is updated in place).  tokens < 2^21, requests <= 2^20,
  * page_size a multiple of 64 up to 4096, pages * page_size < 2^31. */
 int mosaic_paged_step(const int32_t* lengths, const int32_t* add, int32_t* block_table, int64_t table_stride,

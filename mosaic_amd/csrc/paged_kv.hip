@@ -52,6 +52,7 @@ struct StepArgs {
   int32_t *table, *starts, *lengths_out, *seq, *positions, *slots, *count_out;
   int64_t stride;
   int r, pages;
+  uint32_t ids;  // page ids from here on, and below 0, have no slot: it would not fit
   uint32_t width, page, tokens;
 };
 
@@ -132,7 +133,7 @@ __global__ void __launch_bounds__(256) paged_step_kernel(const StepArgs a) {
           else
             id = a.free_pages[free - 1 - ((at[i] ? s_take[at[i] - 1] : taken) + page - old_pages)];
         }
-        slot[i] = placed ? (uint32_t)id * a.page + p % a.page : ~0u;
+        slot[i] = placed && (uint32_t)id < a.ids ? (uint32_t)id * a.page + p % a.page : ~0u;
         if (here) a.positions[t] = placed ? (int32_t)p : -1;
       }
 #pragma unroll
@@ -484,8 +485,8 @@ extern "C" int mosaic_paged_step(const int32_t* lengths, const int32_t* add, int
     for (int o = 0; o < 6; ++o)
       MOSAIC_CHECK_ARG(!overlap(in[i], 4 * in_n[i], out[o], 4 * out_n[o]), "paged_step: an output overlaps an input");
   StepArgs a{lengths, add, free_pages, free_count, block_table, starts, lengths_out, seq_lens, positions, slots,
-             count_out, table_stride, (int)requests, (int)(free_pages ? pages : 0), (uint32_t)width,
-             (uint32_t)page_size, (uint32_t)tokens};
+             count_out, table_stride, (int)requests, (int)(free_pages ? pages : 0),
+             (uint32_t)((1ll << 31) / page_size), (uint32_t)width, (uint32_t)page_size, (uint32_t)tokens};
   const unsigned grid = (unsigned)(tokens > kRows ? (tokens + kRows - 1) / kRows : 1);
   // one request a thread is read at once (16 requests: 4.4 us, with eight 6.5), eight
   // need one scan for 2048 of them (in two of 1024: 11.4 us, so 9.3)

@@ -42,7 +42,8 @@ def step(lengths, new, table, tokens, page, free=None, count=0):
         for t in range(n):
             p = held + t
             positions[begin + t] = p
-            slots[begin + t] = table[i, p // page] * page + p % page
+            if 0 <= table[i, p // page] < 2 ** 31 // page:
+                slots[begin + t] = table[i, p // page] * page + p % page
     return dict(starts=starts, lengths=lengths_out, seq_lens=seq, positions=positions, slots=slots,
                 free_count=np.array([left], np.int32))
 

@@ -823,3 +823,25 @@ def test_attention_values_past_the_range_reach_only_rows_that_see_them(dev, held
     for i in range(len(held)):
         s[table[i, 1], 0, 0, 0] = 240  # the same key, its score far below but finite
     np.testing.assert_array_equal(_attend(dev, q, c, s, table, starts, seq, 0.125)[:, 1], o[:, 1])
+
+
+# -------------------------------------------- the pool's edges and promises ----
+def test_slots_of_pages_outside_the_pool(dev):
+    """An id below 0, or whose slots would pass 31 bits, gives its rows none, from the stack as from a table."""
+    from mosaic_amd import ops
+    free = np.array([3, -1, 9, 1 << 30, 4], np.int32)
+    table = np.zeros((3, 4), np.int32)
+    lengths, new = np.array([0, 0, 0], np.int32), np.array([100, 130, 5], np.int32)
+    count = 5
+    t = _i32(table, dev)
+    s = ops.paged_step(_i32(lengths, dev), _i32(new, dev), t, 235, 64, _i32(free, dev), _i32([count], dev))
+    slots, pos = s.slots.cpu().numpy(), s.positions.cpu().numpy()
+    assert pos[:100].tolist() == list(range(100))
+    assert slots[:64].tolist() == list(range(4 * 64, 5 * 64)) and (slots[64:100] == -1).all()
+    assert slots[100:164].tolist() == list(range(9 * 64, 10 * 64)) and (slots[164:228] == -1).all()
+    assert slots[228:230].tolist() == [3 * 64, 3 * 64 + 1] and (slots[230:] == -1).all()
+    given = _i32([[-7, 5, 1 << 26, 0]], dev)
+    s = ops.paged_step(_i32([10], dev), _i32([200], dev), given, 200, 64)
+    slots = s.slots.cpu().numpy()
+    assert (slots[:54] == -1).all() and slots[54:118].tolist() == list(range(320, 384)) and (slots[118:182] == -1).all()
+    assert slots[182:].tolist() == list(range(18))
