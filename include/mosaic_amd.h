@@ -553,8 +553,8 @@ int mosaic_dsa_decode_indices(const int32_t* pos, int64_t rows, int64_t window, 
  * request: its rows attend to nothing and give zeros); positions and slots
  * [tokens] (page id * page_size + offset; -1 for rows that are not placed or
  * behind the last request, and slots of -1 where the table's id is below 0 or the
- * slot not below 2^31); *count_out: pages left.  Outputs may not overlap
- * inputs (block_table is updated in place).  tokens < 2^21, requests <= 2^20,
+ * slot not below 2^31); *count_out: pages left.  Outputs may overlap
+ * neither inputs nor each other, block_table, which is updated in place, none of them.  tokens < 2^21, requests <= 2^20,
  * page_size a multiple of 64 up to 4096, pages * page_size < 2^31. */
 int mosaic_paged_step(const int32_t* lengths, const int32_t* add, int32_t* block_table, int64_t table_stride,
                       const int32_t* free_pages, const int32_t* free_count, int64_t requests, int64_t width,
@@ -564,8 +564,8 @@ int mosaic_paged_step(const int32_t* lengths, const int32_t* add, int32_t* block
 /* Shortens requests to keep[r] tokens (0 releases one; more than it holds
  * changes nothing) and pushes the pages behind them, the last request's last
  * page first: the inverse of a step.  `pages` is the stack's capacity; the
- * tables, of fewer than 2^31 entries, are left as they are.  lengths_out and count_out may not overlap the
- * inputs (free_pages is updated in place). */
+ * tables, of fewer than 2^31 entries, are left as they are.  lengths_out and count_out may overlap neither the
+ * inputs nor each other, free_pages, which is updated in place, none of them. */
 int mosaic_paged_trim(const int32_t* lengths, const int32_t* keep, const int32_t* block_table, int64_t table_stride,
                       int32_t* free_pages, const int32_t* free_count, int64_t requests, int64_t width, int64_t pages,
                       int64_t page_size, int32_t* lengths_out, int32_t* count_out, void* stream);

@@ -451,7 +451,14 @@ __global__ void __launch_bounds__(256) paged_kv_write_kernel(const WriteArgs a) 
 
 bool overlap(const void* a, int64_t na, const void* b, int64_t nb) {
   const char *x = (const char*)a, *y = (const char*)b;
-  return x && y && x < y + nb && y < x + na;
+  return x && y && na && nb && x < y + nb && y < x + na;
+}
+// the rows of a table, not what lies between them
+bool overlap(const int32_t* table, int64_t rows, int64_t width, int64_t stride, const int32_t* b, int64_t n) {
+  const int64_t at = ((intptr_t)b - (intptr_t)table) / 4;  // the last row that begins in front of b, or the first
+  const int64_t row = at <= 0 || rows == 0 ? 0 : at / stride < rows ? at / stride : rows - 1;
+  return table && rows && (overlap(table + row * stride, 4 * width, b, 4 * n) ||
+                           (row + 1 < rows && overlap(table + (row + 1) * stride, 4 * width, b, 4 * n)));
 }
 
 }  // namespace
@@ -484,6 +491,15 @@ extern "C" int mosaic_paged_step(const int32_t* lengths, const int32_t* add, int
   for (int i = 0; i < 4; ++i)
     for (int o = 0; o < 6; ++o)
       MOSAIC_CHECK_ARG(!overlap(in[i], 4 * in_n[i], out[o], 4 * out_n[o]), "paged_step: an output overlaps an input");
+  for (int o = 0; o < 6; ++o) {
+    for (int i = 0; i < o; ++i)
+      MOSAIC_CHECK_ARG(!overlap(out[i], 4 * out_n[i], out[o], 4 * out_n[o]), "paged_step: an output overlaps another");
+    MOSAIC_CHECK_ARG(!overlap(block_table, requests, width, table_stride, out[o], out_n[o]),
+                     "paged_step: an output overlaps the tables");
+  }
+  for (int i = 0; free_pages && i < 4; ++i)
+    MOSAIC_CHECK_ARG(!overlap(block_table, requests, width, table_stride, in[i], in_n[i]),
+                     "paged_step: the tables overlap an input");
   StepArgs a{lengths, add, free_pages, free_count, block_table, starts, lengths_out, seq_lens, positions, slots,
              count_out, table_stride, (int)requests, (int)(free_pages ? pages : 0),
              (uint32_t)((1ll << 31) / page_size), (uint32_t)width, (uint32_t)page_size, (uint32_t)tokens};
@@ -521,6 +537,12 @@ extern "C" int mosaic_paged_trim(const int32_t* lengths, const int32_t* keep, co
   for (int i = 0; i < 3; ++i)
     for (int o = 0; o < 3; ++o)
       MOSAIC_CHECK_ARG(!overlap(in[i], 4 * in_n[i], out[o], 4 * out_n[o]), "paged_trim: an output overlaps an input");
+  for (int o = 0; o < 3; ++o) {
+    for (int i = 0; i < o; ++i)
+      MOSAIC_CHECK_ARG(!overlap(out[i], 4 * out_n[i], out[o], 4 * out_n[o]), "paged_trim: an output overlaps another");
+    MOSAIC_CHECK_ARG(!overlap(block_table, requests, width, table_stride, out[o], out_n[o]),
+                     "paged_trim: an output overlaps the tables");
+  }
   TrimArgs a{lengths, keep, block_table, free_count, free_pages, lengths_out, count_out, table_stride,
              (int)requests, (int)pages, (uint32_t)width, (uint32_t)page_size};
   const int64_t most = (pages < requests * width ? pages : requests * width) / 1024;

@@ -203,3 +203,36 @@ def test_wrappers_refuse_cpu_tensors_and_bad_caches():
 def test_trim_refuses_tables_whose_pages_pass_32_bits(r, width):
     """Lengths that claim whole tables would make the count of freed pages wrap, and columns be read outside a row."""
     _refused("mosaic_paged_trim", _trim(r=r, width=width, stride=width), "entries")
+
+
+def _at(page, word=0):
+    return ctypes.c_void_p((page << 12) + 4 * word)
+
+
+@pytest.mark.parametrize("kw,text", [
+    (dict(out=_at(3, 1)), "overlaps the tables"), (dict(pos=_at(3, 7)), "overlaps the tables"),
+    (dict(slots=_at(3, 999), stride=1000), "overlaps the tables"), (dict(left=_at(3, 1003), stride=1000), "overlaps the tables"),
+    (dict(table=_at(1, 1)), "tables overlap"), (dict(table=_at(2, -1000), stride=1000), "tables overlap"),
+    (dict(table=_at(4, -3)), "tables overlap"), (dict(table=_at(5)), "tables overlap"),
+    (dict(seq=_at(7, 1)), "overlaps another"), (dict(slots=_at(9, -1)), "overlaps another"),
+    (dict(left=_at(6, 2)), "overlaps another")])
+def test_step_refuses_shared_memory(kw, text):
+    _refused("mosaic_paged_step", _step(**kw), text)
+
+
+@pytest.mark.parametrize("kw,text", [
+    (dict(out=_at(3, 7)), "overlaps the tables"), (dict(free=_at(3, -7)), "overlaps the tables"),
+    (dict(left=_at(3, 1001), stride=1000), "overlaps the tables"), (dict(left=_at(6, 1)), "overlaps another"),
+    (dict(out=_at(4, 7)), "overlaps another")])
+def test_trim_refuses_shared_memory(kw, text):
+    _refused("mosaic_paged_trim", _trim(**kw), text)
+
+
+@pytest.mark.parametrize("kw", [dict(out=_at(3, 4), stride=1000), dict(out=_at(3, 998), stride=1000), dict(pos=_at(3, 1004), stride=1000),
+                                dict(table=_at(1, 2), free=None, count=None)])
+def test_step_takes_what_lies_between_the_rows(kw):
+    """Memory between a table's rows is another's, and one that nothing is written to may be an input too: these
+    calls pass the checks (what fails is the launch, without a GPU)."""
+    if torch.cuda.is_available():
+        pytest.skip("the pointers are made up")
+    assert _lib.lib().mosaic_paged_step(*_step(**kw)) > 0
