@@ -1091,6 +1091,7 @@ def paged_step(lengths: torch.Tensor, new: torch.Tensor, block_table: torch.Tens
     if free_pages is not None:
         pages = free_pages.numel() if isinstance(free_pages, torch.Tensor) else 0
         free, count = _index(free_pages, "free_pages", pages, dev), _index(free_count, "free_count", 1, dev)
+        free = free or count  # a pool of no pages has no address; nothing of it is read
     tokens = int(tokens)
     at, add = _index(lengths, "lengths", r, dev), _index(new, "new", r, dev)
     table, stride, width = _table(block_table, r, dev)

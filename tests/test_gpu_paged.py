@@ -845,3 +845,10 @@ def test_slots_of_pages_outside_the_pool(dev):
     slots = s.slots.cpu().numpy()
     assert (slots[:54] == -1).all() and slots[54:118].tolist() == list(range(320, 384)) and (slots[118:182] == -1).all()
     assert slots[182:].tolist() == list(range(18))
+
+
+def test_step_with_an_empty_pool(dev):
+    """A pool of no pages places what needs none."""
+    from mosaic_amd import ops
+    s = ops.paged_step(_i32([3, 64], dev), _i32([2, 1], dev), _i32([[7, 7], [8, 8]], dev), 3, 64, _i32([], dev), _i32([0], dev))
+    assert s.seq_lens.tolist() == [5, 0] and s.lengths.tolist() == [5, 64] and s.free_count.tolist() == [0]
