@@ -544,7 +544,9 @@ int mosaic_dsa_decode_indices(const int32_t* pos, int64_t rows, int64_t window, 
 /* Block tables and slot map of one step.  lengths [requests]: tokens that each
  * request holds; add [requests]: tokens that this step adds (negative: none).
  * Requests are placed in order; one is not placed where its rows pass `tokens`,
- * its tokens pass its table row, or the pool has too few pages left.  A placed
+ * its tokens pass its table row, or it needs pages and the stack holds too few for
+ * it and all before it whose rows and tokens fit, placed or not: once pages do not
+ * suffice, no later request that needs one is placed.  A placed
  * request's new pages are popped from the stack free_pages[0 .. *free_count)
  * (top: the last one) into its table row; with free_pages NULL the tables hold
  * them already.  Outputs: starts [requests + 1] (the prefix of add, placed or

@@ -1081,8 +1081,11 @@ def paged_step(lengths: torch.Tensor, new: torch.Tensor, block_table: torch.Tens
     (``free_count`` [1] of them) into ``block_table`` [R, B], which is updated in
     place; without ``free_pages`` the tables hold the pages already.  Requests
     are placed in order; one whose rows, table or pages do not suffice is not
-    placed: its length stays, its ``seq_lens`` is 0, its rows have no slot.  The
-    inputs other than the table are left as they are (``out`` may not share
+    placed: its length stays, its ``seq_lens`` is 0, its rows have no slot.  Pages
+    are handed out first come, first served: once one request gets too few, no
+    later one that needs a page is placed either, however many are left, and those
+    that need none are (leave the large one out of ``new``, or put it last, to let
+    the others go on).  The inputs other than the table are left as they are (``out`` may not share
     their memory): commit a step by copying ``lengths`` and ``free_count``."""
     dev, r = _requests(lengths, "lengths")
     if (free_pages is None) != (free_count is None):

@@ -852,3 +852,14 @@ def test_step_with_an_empty_pool(dev):
     from mosaic_amd import ops
     s = ops.paged_step(_i32([3, 64], dev), _i32([2, 1], dev), _i32([[7, 7], [8, 8]], dev), 3, 64, _i32([], dev), _i32([0], dev))
     assert s.seq_lens.tolist() == [5, 0] and s.lengths.tolist() == [5, 64] and s.free_count.tolist() == [0]
+
+
+def test_step_refuses_in_order(dev):
+    """Pages are handed out in the order of the requests: one that gets too few keeps later ones from theirs, but
+    not those that need none."""
+    from mosaic_amd import ops
+    lengths, new = [10, 60, 64, 64, 5], [1, 600, 1, 0, 2]  # pages needed: 0, 10, 1, 0, 0
+    table = _i32(np.tile(np.arange(16), (5, 1)), dev)
+    s = ops.paged_step(_i32(lengths, dev), _i32(new, dev), table, 604, 64, _i32([20, 21, 22], dev), _i32([3], dev))
+    assert s.seq_lens.tolist() == [11, 0, 0, 64, 7]
+    assert s.lengths.tolist() == [11, 60, 64, 64, 7] and s.free_count.tolist() == [3]
