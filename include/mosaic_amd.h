@@ -565,7 +565,10 @@ int mosaic_paged_step(const int32_t* lengths, const int32_t* add, int32_t* block
 
 /* Shortens requests to keep[r] tokens (0 releases one; more than it holds
  * changes nothing) and pushes the pages behind them, the last request's last
- * page first: the inverse of a step.  `pages` is the stack's capacity; the
+ * page first: the inverse of a step.  Ids are pushed as the tables hold them: each has
+ * to be a page of the pool and no other request's.  Where the first pages are shared,
+ * keep is their tokens, and the caller takes the request's length to 0 itself; their
+ * last owner alone releases them.  `pages` is the stack's capacity; the
  * tables, of fewer than 2^31 entries, are left as they are.  lengths_out and count_out may overlap neither the
  * inputs nor each other, free_pages, which is updated in place, none of them. */
 int mosaic_paged_trim(const int32_t* lengths, const int32_t* keep, const int32_t* block_table, int64_t table_stride,

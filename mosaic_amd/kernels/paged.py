@@ -71,7 +71,8 @@ class PagedKVCache:
         return self.attend(step, q, softmax_scale, sink, window, max_new, layer, workspace)
 
     def trim(self, keep: torch.Tensor) -> None:
-        """Shorten request r to ``keep[r]`` tokens (0 releases it) and take its pages back."""
+        """Shorten request r to ``keep[r]`` tokens (0 releases it) and take its pages back, which have to be
+        its own: keep those of a prefix that it shares (``ops.paged_trim``)."""
         lengths, count = ops.paged_trim(self.lengths, keep, self.block_table, self.page_size, self.free_pages,
                                         self.free_count)
         self.lengths.copy_(lengths)

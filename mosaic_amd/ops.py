@@ -1116,7 +1116,12 @@ def paged_trim(lengths: torch.Tensor, keep: torch.Tensor, block_table: torch.Ten
                free_pages: torch.Tensor, free_count: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """Shorten requests to ``keep[r]`` tokens (0 releases one; more than it holds
     changes nothing) and push the pages behind them onto ``free_pages``, in
-    place: the inverse of ``paged_step``.  -> (lengths [R], free_count [1])."""
+    place: the inverse of ``paged_step``.  -> (lengths [R], free_count [1]).
+    What is pushed has to be a page of the pool and this request's alone: ids are
+    taken as the tables hold them, and a page that others still read, or that two
+    requests give back, would be handed out while it is in use.  A request whose
+    first pages are shared (whole pages: a common prefix) is shortened to those,
+    and its length then set to 0; the last one that holds them releases them."""
     dev, r = _requests(lengths, "lengths")
     if not isinstance(free_pages, torch.Tensor):
         raise TypeError(f"free_pages must be a torch.Tensor, got {type(free_pages).__name__}")
@@ -1200,7 +1205,8 @@ def paged_attention(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, 
     scores are all -inf is not a number, or zero beside a sink.  ``max_new``:
     the most rows of any request where the caller knows it (it only sizes the
     launches).  ``starts`` ascends from 0.  ``out`` may not overlap q.  Requests may
-    share pages (a common prefix).  A ``workspace`` serves one call at a time: calls on other
+    share pages that they only read (a common prefix; see ``paged_trim`` for their
+    release).  A ``workspace`` serves one call at a time: calls on other
     streams, and graphs that may replay at once, need one each."""
     q, q_at, q_tok, q_head = _paged_rows(q, "q")
     dev = q.get_device()

@@ -863,3 +863,19 @@ def test_step_refuses_in_order(dev):
     s = ops.paged_step(_i32(lengths, dev), _i32(new, dev), table, 604, 64, _i32([20, 21, 22], dev), _i32([3], dev))
     assert s.seq_lens.tolist() == [11, 0, 0, 64, 7]
     assert s.lengths.tolist() == [11, 60, 64, 64, 7] and s.free_count.tolist() == [3]
+
+
+def test_trim_of_requests_that_share_a_prefix(dev):
+    """Each is shortened to the shared pages, which only their last owner gives back: every page is freed once."""
+    from mosaic_amd.kernels.paged import PagedKVCache
+    cache = PagedKVCache(12, 1, 64, 3, 400, device=dev)
+    cache.step(_i32([200, 0, 0], dev), 200)  # four pages, three of them full
+    cache.block_table[1:, :3] = cache.block_table[0, :3]  # two more begin with the full ones
+    cache.lengths[1:] = 192
+    cache.step(_i32([1, 70, 5], dev), 76)
+    assert cache.free_count.tolist() == [12 - 4 - 2 - 1]
+    for keep in ([250, 192, 300], [300, 300, 192], [0, 300, 300]):  # behind the shared pages; the last owner: all
+        cache.trim(_i32(keep, dev))
+        cache.lengths[1:] *= (cache.lengths[1:] != 192)  # the shared ones stay in the pool: no longer this request's
+    assert cache.lengths.tolist() == [0, 0, 0] and cache.free_count.tolist() == [12]
+    assert sorted(cache.free_pages.tolist()) == list(range(12))
