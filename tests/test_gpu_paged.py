@@ -879,3 +879,60 @@ def test_trim_of_requests_that_share_a_prefix(dev):
         cache.lengths[1:] *= (cache.lengths[1:] != 192)  # the shared ones stay in the pool: no longer this request's
     assert cache.lengths.tolist() == [0, 0, 0] and cache.free_count.tolist() == [12]
     assert sorted(cache.free_pages.tolist()) == list(range(12))
+
+
+def _wide(rng, dev, r, pages, hkv, d, width):
+    """A cache and tables so wide that tiles of few rows and of many are cut and joined."""
+    c, s = _cache(rng, pages, 1, hkv, d)
+    return torch.from_numpy(c).to(dev), torch.from_numpy(s).to(dev), _i32(rng.integers(0, pages, (r, width)), dev)
+
+
+def test_cut_tiles_in_a_graph(dev):
+    """Attention that cuts and joins tiles of both kinds, captured once and replayed while lengths and rows change."""
+    from mosaic_amd import ops
+    rng = np.random.default_rng(47)
+    r, t, hq, hkv, d, width = 4, 60, 8, 2, 128, 80
+    c, s, table = _wide(rng, dev, r, 100, hkv, d, width)
+    q = torch.zeros(t, hq, d, dtype=torch.bfloat16, device=dev)
+    starts, seq = _i32(np.zeros(r + 1), dev), _i32(np.zeros(r), dev)
+    ws = ops.MoEWorkspace()
+    args = (q, c, s, table, starts, seq, 0.1)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        ops.paged_attention(*args, workspace=ws)
+    stream.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        o = ops.paged_attention(*args, workspace=ws)
+    for new, held in (([1, 1, 1, 1], [5000, 3, 1200, 0]), ([40, 1, 0, 2], [4900, 5000, 7, 64]), ([0, 0, 0, 0], [9, 9, 9, 9]),
+                      ([4, 4, 4, 4], [100, 200, 5100, 5]), ([50, 1, 2, 3], [0, 4000, 4000, 4000]), ([1, 1, 1, 1], [64, 65, 63, 1])):
+        q.copy_(torch.from_numpy(_bf16(rng, t, hq, d)).to(dev))
+        starts.copy_(_i32(np.concatenate([[0], np.cumsum(new)]), dev))
+        seq.copy_(_i32(np.array(new) + np.array(held), dev))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(o, ops.paged_attention(*args)), new
+
+
+def test_two_streams_at_once(dev):
+    """Calls on two streams, each with a workspace of its own, beside each other over one cache."""
+    from mosaic_amd import ops
+    rng = np.random.default_rng(48)
+    c, s, table = _wide(rng, dev, 3, 60, 2, 64, 90)
+    calls = []
+    for new, held in (([1, 1, 1], [5500, 40, 3000]), ([70, 1, 30], [5000, 2000, 10])):
+        q = torch.from_numpy(_bf16(rng, sum(new), 8, 64)).to(dev).to(torch.bfloat16)
+        calls.append((q, c, s, table, _i32(np.concatenate([[0], np.cumsum(new)]), dev),
+                      _i32(np.array(new) + np.array(held), dev), 0.125))
+    want = [ops.paged_attention(*a) for a in calls]
+    streams, ws = [torch.cuda.Stream() for _ in calls], [ops.MoEWorkspace() for _ in calls]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(ops.paged_attention(*calls[i], workspace=ws[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(x, want[i]) for x in got[i])
